@@ -546,6 +546,89 @@ typedef struct {
 int nsa_decode_step(const nsa_decode_args* args, void* stream);
 
 /* ------------------------------------------------------------------------
+ * Rotation of queries and keys by their positions, alone or behind an RMS
+ * norm of every head, both tensors in one launch, and the gradients (upstream
+ * rotates whole heads of adjacent pairs at NSA:643; partial and half-split
+ * heads, stretched frequencies and norms per head have no counterpart there).
+ *   n = norm ? x * rsqrt(mean(x^2) + eps) * weight : x
+ *   a feature pair (u, v) of n becomes magnitude * (u cos - v sin, v cos + u sin)
+ * at the angle positions[b, i] + offset times the pair's frequency; pairs are
+ * (2m, 2m+1), or (m, m + rotary_dim/2) with `half`; features from rotary_dim
+ * on pass unchanged.  A frequency is given as the 64-bit fraction of a turn
+ * per position (steps[m] = 2^64 * frequency / 2 pi, rounded), so that angles
+ * stay exact at any int64 position.  Any element strides; rows need no
+ * alignment beyond their type's (16-byte aligned ones are moved fastest).
+ * The backward writes dx to `out` and, with norm, the weights' gradients in
+ * the weights' type, in a fixed order of summation.  `out` may be x itself
+ * (or dy), with the same strides, but must not overlap it otherwise.
+ * ---------------------------------------------------------------------- */
+typedef struct {
+  nsa_tensor x;           /* [B, heads, N, d]; backward without norm: not read */
+  nsa_tensor dy;          /* backward only                                     */
+  nsa_tensor out;         /* written                                           */
+  const void* weight;     /* with norm: [d], or [heads, d] with weight_per_head */
+  void* dweight;          /* backward with norm: written                       */
+  int32_t heads;          /* 0: this part is not there                         */
+  int32_t reserved;
+} nsa_head_rows;
+
+typedef struct {
+  nsa_head_rows part[2];  /* queries, keys                                     */
+  const void* positions;  /* [B, N], rows pos_stride_b elements apart (0: one row for all); NULL: 0 .. N-1 */
+  int64_t pos_stride_b;
+  int64_t offset;         /* added to every position                           */
+  const uint64_t* steps;  /* [rotary_dim / 2]                                  */
+  void* workspace;        /* backward with norm: nsa_heads_workspace_bytes     */
+  int64_t workspace_bytes;
+  int32_t batch, seq, dim_head;   /* dim_head even, at most 256                */
+  int32_t rotary_dim;     /* even, 2 .. dim_head                               */
+  int32_t half;           /* pairs (m, m + rotary_dim / 2) instead of (2m, 2m+1) */
+  int32_t norm, weight_f32, weight_per_head;
+  int32_t pos_i64;        /* positions are int64, else int32                   */
+  int32_t dtype;
+  float magnitude, eps;
+} nsa_heads_args;
+
+int64_t nsa_heads_workspace_bytes(const nsa_heads_args* args);
+int nsa_heads_fwd(const nsa_heads_args* args, void* stream);
+int nsa_heads_bwd(const nsa_heads_args* args, void* stream);
+
+/* ------------------------------------------------------------------------
+ * Attention of drafted tokens over a cache, forward only (upstream decodes one
+ * token a step, NSA:387-547; there is no counterpart for several).  Token t of
+ * sequence b attends the first lengths[b] rows of the cache, all of them, and
+ * the drafted rows u with mask[b, t, u] != 0 (its ancestors and itself, for a
+ * tree; without a mask all u <= t):
+ *   out = sum_j p_j v_j,  p = softmax(scale * q . k_j),  lse = log sum exp
+ * One token and no mask is plain decoding against a dense cache.  A token that
+ * sees nothing gets zeros and lse = -inf.  Rows of the cache behind a length,
+ * and drafted rows a token does not see, leave no trace in it whatever they
+ * hold, NaN included.  Lengths are read on the device and held to
+ * 0 .. capacity.  Any strides in elements; the tensor-core kernel (bf16) wants
+ * rows of k, v and the caches on 16-byte boundaries, the other serves the rest.
+ * ---------------------------------------------------------------------- */
+typedef struct {
+  nsa_tensor q;            /* [B, q_heads, T, d]                               */
+  nsa_tensor k_cache, v_cache;   /* [B, kv_heads, capacity, d]                 */
+  nsa_tensor k, v;         /* [B, kv_heads, T, d], of the drafted tokens       */
+  nsa_tensor out;          /* [B, q_heads, T, d] written                       */
+  float* lse;              /* [B, q_heads, T] written, or NULL                 */
+  const int32_t* lengths;  /* [B] on the device, or NULL: `length` for all     */
+  const uint8_t* mask;     /* [B, T, T], last axis contiguous, or NULL         */
+  int64_t mask_stride_b, mask_stride_t;   /* stride_b 0: one tree for all      */
+  void* workspace;         /* nsa_tree_workspace_bytes(args), 256-byte aligned */
+  int64_t workspace_bytes;
+  int32_t* status;         /* the device word the tensor-core kernel ORs its status into, or NULL */
+  int32_t batch, q_heads, kv_heads, tokens, dim_head;
+  int32_t capacity, length;
+  int32_t dtype, impl;     /* NSA_F32 / NSA_BF16, NSA_IMPL_*                   */
+  float scale;
+} nsa_tree_args;
+
+int64_t nsa_tree_workspace_bytes(const nsa_tree_args* args);
+int nsa_tree_attend(const nsa_tree_args* args, void* stream);
+
+/* ------------------------------------------------------------------------
  * Housekeeping (no counterparts in upstream).
  * ---------------------------------------------------------------------- */
 
@@ -565,7 +648,8 @@ int nsa_selftest_bounded_wait(int* status_device, int64_t limit_cycles, void* st
 /* Library information.  nsa_struct_size(i) is sizeof() of the i-th argument
  * struct in declaration order (0 nsa_tensor, 1 sel_fwd, 2 sel_bwd, 3 cmp_fwd,
  * 4 cmp_bwd, 5 select, 6 swa_fwd, 7 swa_bwd, 8 combine_fwd, 9 combine_bwd, 10 combine_gather,
- * 11 rotary, 12 windows_fwd, 13 windows_bwd, 14 rmsnorm_fwd, 15 rmsnorm_bwd, 16 decode), so
+ * 11 rotary, 12 windows_fwd, 13 windows_bwd, 14 rmsnorm_fwd, 15 rmsnorm_bwd, 16 decode,
+ * 17 head_rows, 18 heads, 19 tree), so
  * a foreign-function binding can verify its own layout; -1 for other i. */
 const char* nsa_last_error(void);
 int nsa_abi_version(void);

@@ -121,14 +121,35 @@ class DecodeArgs(C.Structure):
                 ('reserved', i32)]
 
 
+class HeadRows(C.Structure):
+    _fields_ = [('x', Tensor4), ('dy', Tensor4), ('out', Tensor4), ('weight', vp), ('dweight', vp), ('heads', i32),
+                ('reserved', i32)]
+
+
+class HeadsArgs(C.Structure):
+    _fields_ = [('part', HeadRows * 2), ('positions', vp), ('pos_stride_b', i64), ('offset', i64), ('steps', vp),
+                ('workspace', vp), ('workspace_bytes', i64), ('batch', i32), ('seq', i32), ('dim_head', i32),
+                ('rotary_dim', i32), ('half', i32), ('norm', i32), ('weight_f32', i32), ('weight_per_head', i32),
+                ('pos_i64', i32), ('dtype', i32), ('magnitude', f32), ('eps', f32)]
+
+
+class TreeArgs(C.Structure):
+    _fields_ = [('q', Tensor4), ('k_cache', Tensor4), ('v_cache', Tensor4), ('k', Tensor4), ('v', Tensor4),
+                ('out', Tensor4), ('lse', vp), ('lengths', vp), ('mask', vp), ('mask_stride_b', i64),
+                ('mask_stride_t', i64), ('workspace', vp), ('workspace_bytes', i64), ('status', vp), ('batch', i32),
+                ('q_heads', i32), ('kv_heads', i32), ('tokens', i32), ('dim_head', i32), ('capacity', i32),
+                ('length', i32), ('dtype', i32), ('impl', i32), ('scale', f32)]
+
+
 _STRUCTS = [Tensor4, SelFwdArgs, SelBwdArgs, CmpFwdArgs, CmpBwdArgs, SelectArgs, SwaFwdArgs, SwaBwdArgs,
             CombineFwdArgs, CombineBwdArgs, CombineGatherArgs, RotaryArgs, WindowsFwdArgs, WindowsBwdArgs,
-            RmsNormFwdArgs, RmsNormBwdArgs, DecodeArgs]
+            RmsNormFwdArgs, RmsNormBwdArgs, DecodeArgs, HeadRows, HeadsArgs, TreeArgs]
 
 ENTRY_POINTS = ['nsa_sel_fwd', 'nsa_sel_bwd', 'nsa_sel_workspace_bytes', 'nsa_sel_index_bytes', 'nsa_cmp_index_bytes', 'nsa_swa_index_bytes', 'nsa_sel_bwd_stores_dq', 'nsa_cmp_bwd_stores_dq', 'nsa_swa_bwd_stores_dq',
                 'nsa_sel_fwd_static', 'nsa_sel_static_status', 'nsa_launch_count', 'nsa_selftest_bounded_wait', 'nsa_decode_step',
                 'nsa_sel_static_scratch_bytes', 'nsa_cmp_workspace_bytes', 'nsa_swa_workspace_bytes', 'nsa_cmp_fwd', 'nsa_cmp_fwd_pools', 'nsa_cmp_bwd', 'nsa_select',
-                'nsa_swa_fwd', 'nsa_swa_bwd', 'nsa_combine_fwd', 'nsa_combine_bwd', 'nsa_combine_fwd_gather', 'nsa_sel_fwd_combine_gather', 'nsa_rotary', 'nsa_windows_fwd', 'nsa_windows_bwd', 'nsa_rmsnorm_fwd', 'nsa_rmsnorm_bwd', 'nsa_last_error',
+                'nsa_swa_fwd', 'nsa_swa_bwd', 'nsa_combine_fwd', 'nsa_combine_bwd', 'nsa_combine_fwd_gather', 'nsa_sel_fwd_combine_gather', 'nsa_rotary', 'nsa_windows_fwd', 'nsa_windows_bwd', 'nsa_rmsnorm_fwd', 'nsa_rmsnorm_bwd',
+                'nsa_heads_workspace_bytes', 'nsa_heads_fwd', 'nsa_heads_bwd', 'nsa_tree_workspace_bytes', 'nsa_tree_attend', 'nsa_last_error',
                 'nsa_abi_version', 'nsa_struct_size']
 
 _lib = None
@@ -159,6 +180,8 @@ def load():
     lib.nsa_selftest_bounded_wait.argtypes = [vp, i64, vp]
     lib.nsa_cmp_workspace_bytes.restype = i64
     lib.nsa_swa_workspace_bytes.restype = i64
+    lib.nsa_heads_workspace_bytes.restype = i64
+    lib.nsa_tree_workspace_bytes.restype = i64
     for which, st in enumerate(_STRUCTS):
         if lib.nsa_struct_size(which) != C.sizeof(st):
             raise NsaError(f'struct layout mismatch for {st.__name__}: library {lib.nsa_struct_size(which)} '

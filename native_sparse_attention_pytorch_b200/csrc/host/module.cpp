@@ -31,4 +31,6 @@ PYBIND11_MODULE(_nsa_host, m) {
   nsa_host::bind_selected(m);
   nsa_host::bind_decode(m);
   nsa_host::bind_layer(m);
+  nsa_host::bind_heads(m);
+  nsa_host::bind_tree(m);
 }

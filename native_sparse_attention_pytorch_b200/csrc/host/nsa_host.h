@@ -90,5 +90,7 @@ void bind_status(pybind11::module_& m);
 void bind_selected(pybind11::module_& m);
 void bind_decode(pybind11::module_& m);
 void bind_layer(pybind11::module_& m);
+void bind_heads(pybind11::module_& m);
+void bind_tree(pybind11::module_& m);
 
 }  // namespace nsa_host

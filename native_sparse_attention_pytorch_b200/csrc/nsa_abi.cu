@@ -157,6 +157,9 @@ int nsa_struct_size(int which) {
     case 14: return (int)sizeof(nsa_rmsnorm_fwd_args);
     case 15: return (int)sizeof(nsa_rmsnorm_bwd_args);
     case 16: return (int)sizeof(nsa_decode_args);
+    case 17: return (int)sizeof(nsa_head_rows);
+    case 18: return (int)sizeof(nsa_heads_args);
+    case 19: return (int)sizeof(nsa_tree_args);
     default: return -1;
   }
 }
@@ -671,6 +674,120 @@ int nsa_rmsnorm_bwd(const nsa_rmsnorm_bwd_args* a, void* stream) {
   }
   P.dy = a->dy; P.dx = a->dx; P.dweight = a->dweight;
   return launch_rmsnorm(P, a->fwd.dtype, true, (cudaStream_t)stream);
+}
+
+static int fill_heads(HeadsParams& P, const nsa_heads_args& a, bool backward) {
+  if (a.dtype != NSA_F32 && a.dtype != NSA_BF16) return fail(NSA_ERR_DTYPE, "dtype must be NSA_F32 or NSA_BF16");
+  if (a.batch < 0 || a.seq < 0 || a.part[0].heads < 0 || a.part[1].heads < 0)
+    return fail(NSA_ERR_SHAPE, "heads: negative size");
+  if (a.dim_head < 2 || a.dim_head % 2 || a.dim_head > kHeadsMaxDim)
+    return fail(NSA_ERR_SHAPE, "heads: dim_head must be even and at most 256");
+  if (a.rotary_dim < 2 || a.rotary_dim % 2 || a.rotary_dim > a.dim_head)
+    return fail(NSA_ERR_SHAPE, "heads: rotary_dim must be even, at least 2 and at most dim_head");
+  if ((int64_t)a.batch * a.seq > 0x7fffffffLL) return fail(NSA_ERR_SHAPE, "heads: batch * seq must stay below 2^31");
+  memset(&P, 0, sizeof(P));
+  P.batch = a.batch; P.seq = a.seq; P.d = a.dim_head; P.rotary_dim = a.rotary_dim; P.half = a.half != 0;
+  P.norm = a.norm != 0; P.weight_f32 = a.weight_f32 != 0; P.weight_per_head = a.weight_per_head != 0;
+  P.positions = a.positions; P.pos_sb = a.pos_stride_b; P.pos_i64 = a.pos_i64 != 0; P.offset = a.offset;
+  P.steps = a.steps; P.magnitude = a.magnitude; P.eps = a.eps;
+  const bool rows = (int64_t)a.batch * a.seq > 0;
+  if (rows && a.steps == nullptr) return fail(NSA_ERR_NULL, "heads: steps is NULL");
+  const uintptr_t unit = a.dtype == NSA_F32 ? 3 : 1;
+  for (int i = 0; i < 2; ++i) {
+    const nsa_head_rows& r = a.part[i];
+    if (r.heads == 0) continue;
+    HeadRows& R = P.part[i];
+    R.heads = r.heads;
+    R.weight = r.weight; R.dweight = r.dweight;
+    if (a.norm && (rows && r.weight == nullptr)) return fail(NSA_ERR_NULL, "heads: weight is NULL");
+    if (a.norm && backward && r.dweight == nullptr) return fail(NSA_ERR_NULL, "heads: dweight is NULL");
+    if (!rows) continue;
+    const bool reads_x = !backward || a.norm;
+    if (r.out.ptr == nullptr || (reads_x && r.x.ptr == nullptr) || (backward && r.dy.ptr == nullptr))
+      return fail(NSA_ERR_NULL, "heads: NULL pointer");
+    const uintptr_t at = reinterpret_cast<uintptr_t>(r.out.ptr) | (reads_x ? reinterpret_cast<uintptr_t>(r.x.ptr) : 0) |
+                         (backward ? reinterpret_cast<uintptr_t>(r.dy.ptr) : 0);
+    if (at & unit) return fail(NSA_ERR_ALIGN, "heads: a tensor does not start on a boundary of its type");
+    R.out = r.out.ptr; R.o_sb = r.out.stride_b; R.o_sh = r.out.stride_h; R.o_sn = r.out.stride_n;
+    if (reads_x) { R.x = r.x.ptr; R.x_sb = r.x.stride_b; R.x_sh = r.x.stride_h; R.x_sn = r.x.stride_n; }
+    if (backward) { R.dy = r.dy.ptr; R.dy_sb = r.dy.stride_b; R.dy_sh = r.dy.stride_h; R.dy_sn = r.dy.stride_n; }
+  }
+  return NSA_OK;
+}
+
+int64_t nsa_heads_workspace_bytes(const nsa_heads_args* a) {
+  if (a == nullptr) return fail(NSA_ERR_NULL, "args: NULL pointer");
+  HeadsParams P;
+  memset(&P, 0, sizeof(P));
+  P.norm = a->norm != 0; P.d = a->dim_head; P.part[0].heads = a->part[0].heads; P.part[1].heads = a->part[1].heads;
+  return heads_partial_floats(P) * (int64_t)sizeof(float);
+}
+
+int nsa_heads_fwd(const nsa_heads_args* a, void* stream) {
+  if (a == nullptr) return fail(NSA_ERR_NULL, "args: NULL pointer");
+  HeadsParams P;
+  NSA_TRY(fill_heads(P, *a, false));
+  if (P.part[0].heads + P.part[1].heads == 0) return NSA_OK;
+  return launch_heads(P, a->dtype, false, (cudaStream_t)stream);
+}
+
+int nsa_heads_bwd(const nsa_heads_args* a, void* stream) {
+  if (a == nullptr) return fail(NSA_ERR_NULL, "args: NULL pointer");
+  HeadsParams P;
+  NSA_TRY(fill_heads(P, *a, true));
+  if (P.part[0].heads + P.part[1].heads == 0) return NSA_OK;
+  if (P.norm && (int64_t)a->batch * a->seq > 0) {
+    if (a->workspace == nullptr || a->workspace_bytes < nsa_heads_workspace_bytes(a) || (reinterpret_cast<uintptr_t>(a->workspace) & 3u))
+      return fail(NSA_ERR_WORKSPACE, "heads: the work buffer is missing, too small or not aligned");
+    P.partial = static_cast<float*>(a->workspace);
+  }
+  return launch_heads(P, a->dtype, true, (cudaStream_t)stream);
+}
+
+// ---- attention of drafted tokens over a cache --------------------------------------
+
+static int fill_tree(TreeParams& P, const nsa_tree_args& a) {
+  NSA_TRY(check_common(a.dtype, a.batch, a.q_heads, a.kv_heads, a.tokens, a.dim_head));
+  if (a.impl < NSA_IMPL_AUTO || a.impl > NSA_IMPL_SM100) return fail(NSA_ERR_SHAPE, "unknown impl");
+  if (a.capacity < 0) return fail(NSA_ERR_SHAPE, "tree: the cache's capacity is negative");
+  const int64_t rows = (int64_t)(a.q_heads / a.kv_heads) * a.tokens;
+  if (rows > (1 << 24) || (int64_t)a.batch * a.kv_heads > (1 << 24)) return fail(NSA_ERR_SHAPE, "tree: more than 2^24 rows of a KV head, or KV heads");
+  memset(&P, 0, sizeof(P));
+  P.batch = a.batch; P.q_heads = a.q_heads; P.kv_heads = a.kv_heads; P.tokens = a.tokens; P.d = a.dim_head; P.capacity = a.capacity;
+  P.G = a.q_heads / a.kv_heads; P.scale = a.scale; P.length = a.length; P.lengths = a.lengths;
+  P.mask = a.mask; P.m_sb = a.mask_stride_b; P.m_st = a.mask_stride_t; P.lse = a.lse;
+  if ((int64_t)a.batch * a.tokens == 0) return NSA_OK;
+  const nsa_tensor* all[] = {&a.q, &a.k, &a.v, &a.out, &a.k_cache, &a.v_cache};
+  const uintptr_t unit = a.dtype == NSA_F32 ? 3 : 1;
+  for (int i = 0; i < (a.capacity > 0 ? 6 : 4); ++i) {
+    if (all[i]->ptr == nullptr) return fail(NSA_ERR_NULL, "tree: NULL pointer");
+    if (reinterpret_cast<uintptr_t>(all[i]->ptr) & unit) return fail(NSA_ERR_ALIGN, "tree: a tensor does not start on a boundary of its type");
+  }
+  auto set = [](RowView& r, const nsa_tensor& t) { r.p = t.ptr; r.sb = t.stride_b; r.sh = t.stride_h; r.sn = t.stride_n; };
+  set(P.q, a.q); set(P.k, a.k); set(P.v, a.v); set(P.out, a.out);
+  if (a.capacity > 0) { set(P.kc, a.k_cache); set(P.vc, a.v_cache); }
+  return NSA_OK;
+}
+
+int64_t nsa_tree_workspace_bytes(const nsa_tree_args* a) {
+  if (a == nullptr) return fail(NSA_ERR_NULL, "args: NULL pointer");
+  TreeParams P;
+  const int rc = fill_tree(P, *a);
+  if (rc != NSA_OK && rc != NSA_ERR_NULL) return rc;
+  return (int64_t)a->batch * a->tokens == 0 ? 0 : tree_workspace_bytes(P, a->dtype, a->impl);
+}
+
+int nsa_tree_attend(const nsa_tree_args* a, void* stream) {
+  if (a == nullptr) return fail(NSA_ERR_NULL, "args: NULL pointer");
+  TreeParams P;
+  NSA_TRY(fill_tree(P, *a));
+  if ((int64_t)a->batch * a->tokens == 0) return NSA_OK;
+  const int64_t need = tree_workspace_bytes(P, a->dtype, a->impl);
+  if (need < 0) return (int)need;
+  if (need > 0 && (a->workspace == nullptr || a->workspace_bytes < need || (reinterpret_cast<uintptr_t>(a->workspace) & 255u)))
+    return fail(NSA_ERR_WORKSPACE, "tree: the work buffer is missing, too small or not on a 256-byte boundary");
+  P.status = a->status;
+  return launch_tree(P, a->dtype, a->impl, static_cast<uint8_t*>(a->workspace), (cudaStream_t)stream);
 }
 
 }  // extern "C"

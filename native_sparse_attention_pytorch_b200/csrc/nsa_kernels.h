@@ -106,6 +106,52 @@ struct NormParams {
   float eps;
 };
 
+// Rotation of queries and keys, with or without their norm (see nsa_heads.cu)
+constexpr int kHeadsMaxDim = 256;
+struct HeadRows {
+  const void *x, *dy;    // [batch, heads, seq, d]; x is not read by the backward of the rotation alone
+  void* out;             // y, or dx
+  const void* weight;    // [d] or [heads, d]
+  void* dweight;         // the same, in the weight's type
+  int64_t x_sb, x_sh, x_sn, dy_sb, dy_sh, dy_sn, o_sb, o_sh, o_sn;
+  int heads;             // 0: this part is not there
+};
+struct HeadsParams {
+  HeadRows part[2];      // queries, keys
+  const void* positions; // [batch, seq] int64 or int32, rows pos_sb apart, or NULL: 0, 1, ...
+  int64_t pos_sb, offset;
+  const uint64_t* steps; // [rotary_dim / 2]: 2^64 times the turns per position
+  float* partial;        // backward with norm: heads_partial_floats
+  int batch, seq, d, rotary_dim, half, norm, weight_f32, weight_per_head, pos_i64;
+  float magnitude, eps;
+  int lane_shift, per_slot, slots[2];   // filled in by launch_heads
+};
+int64_t heads_partial_floats(const HeadsParams& P);
+int launch_heads(HeadsParams& P, int dtype, bool backward, cudaStream_t stream);
+
+// Attention of drafted tokens over a cache (see nsa_tree.cu)
+struct RowView {
+  const void* p;
+  int64_t sb, sh, sn;
+};
+struct TreeParams {
+  RowView q, k, v, out;    // [B, Hq, T, d], [B, Hkv, T, d] twice, [B, Hq, T, d] written
+  RowView kc, vc;          // [B, Hkv, capacity, d]
+  const int32_t* lengths;  // [B] cached rows, or NULL: `length` of each
+  const uint8_t* mask;     // [B, T, T] with rows m_sb and m_st apart, or NULL: a chain
+  int64_t m_sb, m_st;
+  float* lse;              // [B, Hq, T] or NULL
+  int batch, q_heads, kv_heads, G, tokens, d, capacity, length;
+  float scale;
+  int* status;
+  // filled in by launch_tree
+  float* partial;          // [groups * tiles * 2][tile rows][padded d]
+  float2* stats;           // [groups * tiles * 2][tile rows]: maximum (base 2), sum
+  int tiles, groups;       // row tiles of a KV head; groups of CTAs that share the key blocks out
+};
+int64_t tree_workspace_bytes(const TreeParams& P, int dtype, int impl);
+int launch_tree(TreeParams& P, int dtype, int impl, uint8_t* workspace, cudaStream_t stream);
+
 // One decoding step (see nsa_decode.cu): the newest token's queries against the caches.
 struct DecodeParams {
   const void *q, *qr;            // [B, Hq, d] contiguous: un-rotated / rotated queries of the token

@@ -88,3 +88,14 @@ class RMSNorm(nn.RMSNorm):
         if len(self.normalized_shape) == 1 and rms_norm_supported(x, self.weight) and x.numel() > 0:
             return rms_norm(x, self.weight, self.eps)
         return super().forward(x)
+
+
+def norm_rotate_heads(q, k, q_weight, k_weight, rotary, positions=None, offset=0, eps=None, out=None):
+    """RMS norm of every head of queries and keys and their rotation, in one pass: n = x * rsqrt(mean(x^2) + eps) * weight
+    over the features of a head, then `rotate_heads`.  q [b, q_heads, n, d], k [b, kv_heads, n, d] (or None with its weight);
+    weights [d], or one row per head, [heads, d], both of one form, in the tensors' type or float32.  eps defaults to the
+    machine epsilon of fp32.  The norm is not rounded before the rotation.  Differentiable in q, k and the weights (sums
+    in a fixed order: the same call gives the same gradients); other arguments as `rotate_heads`."""
+    from .rotary import _rotate
+    return _rotate(q, k, q_weight, k_weight, rotary, positions, offset, True,
+                   torch.finfo(torch.float32).eps if eps is None else float(eps), out)

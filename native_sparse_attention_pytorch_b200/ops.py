@@ -707,6 +707,33 @@ def decode_step(q, qr, keys, vals, ck, cv, mem_k, mem_v, gates, *, stride, block
 
 
 # --------------------------------------------------------------------------
+# drafted tokens against a cache
+# --------------------------------------------------------------------------
+
+@torch.no_grad()
+def tree_attend(q, k_cache, v_cache, lengths, k, v, mask=None, *, scale=None, return_lse=False, impl='auto'):
+    """Attention of drafted tokens over a cache and over one another, for verifying a tree of them in one step (or, with one
+    token, for plain decoding against a dense cache; or, without a mask, for a chunk of a prompt).
+
+    q [b, q_heads, t, d], k, v [b, kv_heads, t, d]: the drafted tokens; k_cache, v_cache [b, kv_heads, capacity, d]: rows a
+    sequence has already, of which the first `lengths` count (int32 tensor [b] on the device, read there; or one int; None:
+    all).  mask: bool [t, t] or [b, t, t], mask[.., i, j]: token i sees drafted token j (a tree: its ancestors and itself);
+    None: j <= i.  Every token sees all cached rows.  A token that sees nothing gets zeros and lse -inf; what lies behind a
+    length, or in a drafted row that a token does not see, leaves no trace in it, NaN included.  scale defaults to
+    d^-0.5.  No gradient.  Returns out [b, q_heads, t, d], with `return_lse` also its log sum of exponentials (fp32
+    [b, q_heads, t]), by which it can be merged with attention over other keys.  See nsa_tree_attend in include/nsa_b200.h."""
+    length = k_cache.shape[2] if lengths is None else 0
+    if isinstance(lengths, int):
+        lengths, length = None, lengths
+        if not 0 <= length <= k_cache.shape[2]:
+            raise L.NsaError(f'length must be between 0 and the capacity {k_cache.shape[2]}, got {length}')
+    L.require_cuda(q, k_cache, v_cache, lengths, k, v, mask)
+    out, lse = L.host().tree_attend(q, k_cache, v_cache, lengths, length, k, v, mask, q.shape[-1] ** -0.5 if scale is None else scale,
+                                    return_lse, L.IMPL_BY_NAME[impl], _status_word(q.device))
+    return (out, lse) if return_lse else out
+
+
+# --------------------------------------------------------------------------
 # input of the compress networks: windows + intra-block positions (NSA:589-614)
 # --------------------------------------------------------------------------
 

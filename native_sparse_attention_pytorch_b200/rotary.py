@@ -5,10 +5,11 @@ fp32, result in the input dtype.  On CUDA tensors the rotation is one kernel
 of the library (`nsa_rotary`) over tables of cos / sin built here; CPU tensors
 (host-side tests) take the same formula in plain PyTorch."""
 import ctypes as C
+import math
 
 import torch
 from torch import nn
-from torch.autograd import Function
+from torch.autograd import Function, forward_ad
 
 
 _INV_FREQ = {}
@@ -87,3 +88,102 @@ class RotaryEmbedding(nn.Module):
     def rotate_queries_with_cached_keys(self, q, k):
         nq, nk = q.shape[-2], k.shape[-2]
         return self.rotate_queries_or_keys(q, offset=nk - nq), self.rotate_queries_or_keys(k)
+
+
+LAYOUTS = ('interleaved', 'half')
+SCALINGS = (None, 'linear', 'ntk', 'yarn')
+
+
+class RotaryFrequencies:
+    """The frequencies of a rotary embedding of heads, for `rotate_heads` and `norm_rotate_heads`.
+
+    dim_head      features of a head (even, at most 256); the first `rotary_dim` of them (even; default: all) are rotated
+                  in pairs, the others pass unchanged
+    theta         base: pair m turns by theta^(-2m / rotary_dim) radians a position
+    layout        'interleaved': pairs (2m, 2m+1), as `RotaryEmbedding`; 'half': pairs (m, m + rotary_dim / 2)
+    scaling       for contexts longer than the trained one by `factor`:
+                  'linear'  every frequency divided by factor;
+                  'ntk'     the base becomes theta * factor^(r / (r - 2)), r = rotary_dim: the lowest frequency is divided by
+                            factor, the highest stays;
+                  'yarn'    a pair that makes at least `beta_fast` turns within `original_length` positions keeps its frequency,
+                            one with at most `beta_slow` turns has it divided by factor, linear in the turns between them, and
+                            rotated features are multiplied by 0.1 ln(factor) + 1 (Peng et al. 2023, "YaRN: Efficient Context
+                            Window Extension of Large Language Models", sections 3.2 to 3.4)
+    frequencies   instead of theta and scaling: rotary_dim / 2 radians per position
+    magnitude     factor on the rotated features, instead of the scaling's own
+
+    Frequencies are computed in 64 bits and kept as 64-bit fractions of a turn, so that angles are exact at any position
+    (`module.bfloat16()` of whatever holds this changes nothing)."""
+
+    def __init__(self, dim_head, rotary_dim=None, theta=10000.0, layout='interleaved', scaling=None, factor=1.0,
+                 original_length=None, beta_fast=32.0, beta_slow=1.0, frequencies=None, magnitude=None):
+        rotary_dim = dim_head if rotary_dim is None else rotary_dim
+        if dim_head < 2 or dim_head % 2 or dim_head > 256:
+            raise ValueError(f'dim_head must be even and at most 256, got {dim_head}')
+        if rotary_dim < 2 or rotary_dim % 2 or rotary_dim > dim_head:
+            raise ValueError(f'rotary_dim must be even, at least 2 and at most dim_head, got {rotary_dim}')
+        if layout not in LAYOUTS:
+            raise ValueError(f'layout must be one of {LAYOUTS}, got {layout!r}')
+        if scaling not in SCALINGS:
+            raise ValueError(f'scaling must be one of {SCALINGS}, got {scaling!r}')
+        if not factor > 0 or not theta > 0:
+            raise ValueError(f'theta and factor must be positive, got {theta} and {factor}')
+        if frequencies is not None and scaling is not None:
+            raise ValueError('frequencies are taken as they are: no scaling beside them')
+        if frequencies is None:
+            base = theta * factor ** (rotary_dim / (rotary_dim - 2)) if scaling == 'ntk' and rotary_dim > 2 else theta
+            frequencies = [base ** (-2 * m / rotary_dim) for m in range(rotary_dim // 2)]
+            if scaling == 'linear':
+                frequencies = [f / factor for f in frequencies]
+            elif scaling == 'yarn':
+                if original_length is None or not original_length > 0 or not beta_fast > beta_slow:
+                    raise ValueError('yarn needs original_length, and beta_fast above beta_slow')
+                keep = [min(1., max(0., (original_length * f / (2 * math.pi) - beta_slow) / (beta_fast - beta_slow)))
+                        for f in frequencies]
+                frequencies = [f * k + f / factor * (1 - k) for f, k in zip(frequencies, keep)]
+                if magnitude is None:
+                    magnitude = 0.1 * math.log(factor) + 1.0 if factor > 1 else 1.0
+        frequencies = [float(f) for f in frequencies]
+        if len(frequencies) != rotary_dim // 2 or not all(math.isfinite(f) for f in frequencies):
+            raise ValueError(f'{rotary_dim // 2} finite frequencies are needed, got {len(frequencies)}')
+        self.dim_head, self.rotary_dim, self.layout = dim_head, rotary_dim, layout
+        self.frequencies = tuple(frequencies)
+        self.magnitude = 1.0 if magnitude is None else float(magnitude)
+        # 2^64 times the turns per position; whole turns drop out, and the upper half stands for negative numbers
+        steps = [round(f / (2 * math.pi) * 2.0 ** 64) % 2 ** 64 for f in frequencies]
+        self._steps = torch.tensor([s - 2 ** 64 if s >= 2 ** 63 else s for s in steps], dtype=torch.int64)
+        self._on = {}
+
+    def steps(self, device):
+        """The table on `device`, copied there once."""
+        t = self._on.get(device)
+        if t is None:
+            if torch.cuda.is_current_stream_capturing():
+                from ._lib import NsaError
+                raise NsaError('the frequencies are not on this device yet: call once before a CUDA graph is recorded')
+            t = self._on[device] = self._steps.to(device)
+            torch.cuda.current_stream(device).synchronize()     # other streams may read it from now on
+        return t
+
+
+def _rotate(q, k, q_weight, k_weight, rotary, positions, offset, norm, eps, out):
+    from . import _lib as L
+    for t in (q, k, q_weight, k_weight, positions):
+        L.require_cuda(t)
+    if forward_ad._current_level >= 0:
+        raise L.NsaError('the rotation of heads has no forward-mode derivative')
+    if q.shape[-1] != rotary.dim_head:
+        raise L.NsaError(f'the frequencies are for heads of {rotary.dim_head}, not {q.shape[-1]}')
+    out_q, out_k = (None, None) if out is None else out
+    y, z = L.host().rotate_heads(q, k, q_weight, k_weight, rotary.steps(q.device), rotary.rotary_dim, rotary.layout == 'half',
+                                 rotary.magnitude, positions, offset, norm, eps, out_q, out_k)
+    return y, z
+
+
+def rotate_heads(q, k, rotary, positions=None, offset=0, out=None):
+    """Queries and keys rotated by their positions, in one launch: q [b, q_heads, n, d], k [b, kv_heads, n, d] (or None) ->
+    the same shapes, contiguous; fp32 arithmetic, rounded once.  float32 or bfloat16, any strides with a contiguous last
+    axis.  `positions`: int64 or int32, [n] or [b, n] (default 0 .. n-1), `offset` is added to them.  `out`: a pair of
+    tensors to write instead (rows of a cache, or q and k themselves), where no gradient is wanted.  Differentiable in q and
+    k; gradients keep the memory order of their inputs."""
+    return _rotate(q, k, None, None, rotary, positions, offset, False, 0.0, out)
