@@ -6,6 +6,8 @@
 
 #include "nsa_b200.h"
 
+struct CUtensorMap_st;
+
 namespace nsa {
 
 enum { BR_SEL = 0, BR_CMP = 1, BR_SWA = 2 };
@@ -149,6 +151,9 @@ struct TreeParams {
   float2* stats;           // [groups * tiles * 2][tile rows]: maximum (base 2), sum
   int tiles, groups;       // row tiles of a KV head; groups of CTAs that share the key blocks out
 };
+// A tensor map over bf16 rows (innermost dimension first; 128-byte swizzle, zeros outside), and the device's SMs (nsa_sm100_sel.cu)
+int encode_bf16_tiles(CUtensorMap_st* map, const void* ptr, const uint64_t (&dims)[4], const uint64_t (&strides)[3], const uint32_t (&box)[4]);
+int num_sms();
 int64_t tree_workspace_bytes(const TreeParams& P, int dtype, int impl);
 int launch_tree(TreeParams& P, int dtype, int impl, uint8_t* workspace, cudaStream_t stream);
 

@@ -331,6 +331,33 @@ __device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
   asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
 }
+// The largest of 32 values
+__device__ __forceinline__ float max32(const float (&s)[32]) {
+  float m[4] = {fmaxf(s[0], s[1]), fmaxf(s[2], s[3]), fmaxf(s[4], s[5]), fmaxf(s[6], s[7])};
+#pragma unroll
+  for (int x = 8; x < 32; x += 8)
+#pragma unroll
+    for (int k = 0; k < 4; ++k) m[k] = max3(m[k], s[x + 2 * k], s[x + 2 * k + 1]);
+  return fmaxf(max3(m[0], m[1], m[2]), m[3]);
+}
+// s = 2^(s * scale2 - off) in place; the sum, in fp32 (four partial sums: values x with equal x % 4)
+__device__ __forceinline__ float exp_row32(float (&s)[32], float scale_log2, float off) {
+  const uint64_t scale2 = pack2(scale_log2, scale_log2), off2 = pack2(-off, -off);
+  uint64_t l0 = 0ull, l1 = 0ull;
+#pragma unroll
+  for (int x = 0; x < 32; x += 4) {
+    unpack2(fma2(pack2(s[x], s[x + 1]), scale2, off2), s[x], s[x + 1]);
+    unpack2(fma2(pack2(s[x + 2], s[x + 3]), scale2, off2), s[x + 2], s[x + 3]);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) s[x + k] = ex2(s[x + k]);
+    l0 = add2(l0, pack2(s[x], s[x + 1]));
+    l1 = add2(l1, pack2(s[x + 2], s[x + 3]));
+  }
+  float a, b, c, d;
+  unpack2(l0, a, b);
+  unpack2(l1, c, d);
+  return (a + b) + (c + d);
+}
 __device__ __forceinline__ void red_add_v4(float* addr, float a, float b, float c, float d) {
   asm volatile("red.global.add.v4.f32 [%0], {%1, %2, %3, %4};" ::"l"(addr), "f"(a), "f"(b), "f"(c), "f"(d) : "memory");
 }

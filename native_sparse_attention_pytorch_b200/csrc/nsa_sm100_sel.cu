@@ -384,34 +384,6 @@ __device__ __forceinline__ RowInfo decode_row(uint32_t e, int j, const BlockRule
   return r;
 }
 
-// The largest of 32 values
-__device__ __forceinline__ float max32(const float (&s)[32]) {
-  float m[4] = {fmaxf(s[0], s[1]), fmaxf(s[2], s[3]), fmaxf(s[4], s[5]), fmaxf(s[6], s[7])};
-#pragma unroll
-  for (int x = 8; x < 32; x += 8)
-#pragma unroll
-    for (int k = 0; k < 4; ++k) m[k] = max3(m[k], s[x + 2 * k], s[x + 2 * k + 1]);
-  return fmaxf(max3(m[0], m[1], m[2]), m[3]);
-}
-// s = 2^(s * scale2 - off) in place; the sum, in fp32 (four partial sums: values x with equal x % 4)
-__device__ __forceinline__ float exp_row32(float (&s)[32], float scale_log2, float off) {
-  const uint64_t scale2 = pack2(scale_log2, scale_log2), off2 = pack2(-off, -off);
-  uint64_t l0 = 0ull, l1 = 0ull;
-#pragma unroll
-  for (int x = 0; x < 32; x += 4) {
-    unpack2(fma2(pack2(s[x], s[x + 1]), scale2, off2), s[x], s[x + 1]);
-    unpack2(fma2(pack2(s[x + 2], s[x + 3]), scale2, off2), s[x + 2], s[x + 3]);
-#pragma unroll
-    for (int k = 0; k < 4; ++k) s[x + k] = ex2(s[x + k]);
-    l0 = add2(l0, pack2(s[x], s[x + 1]));
-    l1 = add2(l1, pack2(s[x + 2], s[x + 3]));
-  }
-  float a, b, c, d;
-  unpack2(l0, a, b);
-  unpack2(l1, c, d);
-  return (a + b) + (c + d);
-}
-
 // ---- forward -------------------------------------------------------------------------
 
 // Forward of the selected-block branch.  A CTA of 256 threads walks gather -> S -> softmax -> P V -> store chunk by
@@ -2033,6 +2005,16 @@ static EncodeTiledFn encode_fn() {
   return fn;
 }
 
+int encode_bf16_tiles(CUtensorMap* map, const void* ptr, const uint64_t (&dims)[4], const uint64_t (&strides)[3], const uint32_t (&box)[4]) {
+  EncodeTiledFn enc = encode_fn();
+  if (enc == nullptr) return fail(NSA_ERR_UNSUPPORTED, "cuTensorMapEncodeTiled is not available from this driver");
+  const cuuint32_t es[4] = {1, 1, 1, 1};
+  const cuuint64_t d[4] = {dims[0], dims[1], dims[2], dims[3]}, st[3] = {strides[0], strides[1], strides[2]};
+  const CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(ptr), d, st, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                         CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? NSA_OK : fail(NSA_ERR_UNSUPPORTED, "strides that the tiled format cannot express");
+}
+
 // Tensor map over a [B, H, N, d] bf16 view; one box is a [64 rows x 64 columns] tile of one head.
 static int make_kv_map(CUtensorMap* map, const nsa_tensor& t, int B, int H, int N, int d) {
   EncodeTiledFn enc = encode_fn();
@@ -2161,7 +2143,7 @@ static void fill_params(SelParams& P, const SelProblem& a, const SelPlan& p, uin
   P.pooled = a.pooled; P.cpf = a.cpf > 0 ? a.cpf : 1; P.pool_cols = a.ncb / P.cpf; P.pool_block = P.cpf * a.stride;
 }
 
-static int num_sms() {
+int num_sms() {
   static int n = 0;
   if (n == 0) {
     int dev = 0;

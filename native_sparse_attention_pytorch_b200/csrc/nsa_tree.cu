@@ -129,6 +129,7 @@ __global__ void __launch_bounds__(tree_simt::kThreads, 2) tree_simt_kernel(const
   const int tile = blockIdx.x % P.tiles, group = blockIdx.x / P.tiles;
   const int rows = P.tokens * P.G, row0 = tile * RT;
 
+  ptx::grid_allow_next();
   const int64_t total = total_blocks<kKeys>(P, lane, P.batch);
   const int64_t begin = piece_begin(total, group, P.groups), end = piece_begin(total, group + 1, P.groups);
   if (begin >= end) return;
@@ -317,6 +318,520 @@ __global__ void __launch_bounds__(tree_simt::kThreads, 2) tree_simt_kernel(const
   }
 }
 
+// ---- bf16, on the tensor cores ---------------------------------------------------------------
+
+// A persistent CTA per SM goes through its piece of the key blocks (128 keys):
+//   TMA warp        K and V blocks through a ring of slots (K, V, K, V, ...), across units and as far ahead as the ring holds
+//   mending warp    clears the rows of a V block that lie behind the sequence, and drafted values that are not finite
+//   MMA warp(s)     S = Q K^T, then O += P V with P from tensor memory; one per stream
+//   softmax warps   four per stream, a thread per row (the 32 lanes of tensor memory that a warp reaches): S from tensor memory,
+//                   maximum, exponentials, P back as bf16.  P is rounded (2^-9 on average a weight, as any bf16 tensor of
+//                   weights would be); the sum adds the exponentials as they are.
+// The accumulator O stays in tensor memory.  It is rescaled lazily: a row keeps its reference maximum until a block exceeds it by
+// more than 2^8.
+// SPLIT.  A tensor-core tile has 128 rows however few there are.  Up to 32 rows are written four times over, and warp w takes keys
+// 32 w .. 32 w + 31 of every block for its copy (its P has zeros elsewhere): a quarter of the exponentials a thread, at no cost in
+// products.  Up to 64 rows twice, for halves.  The copies' results are joined in shared memory (in Q's place) where a unit ends.
+// STREAMS.  Above 128 rows two tiles share the K and V blocks; the softmax of one runs under the products of the other.
+namespace tree_tc {
+constexpr int kKeys = 128, kRows = 128;
+template <int D, int STREAMS>
+struct Shape {
+  static constexpr int NC = D / 64;                                // 64-column subtiles of a row
+  static constexpr uint32_t kTile = NC * 16384;                    // Q, K or V: 128 rows
+  static constexpr int kSlots = (14 - STREAMS * NC) / NC;          // 14 tiles of 16 KB fit
+  static constexpr uint32_t kBytes = (STREAMS + kSlots) * kTile;
+  static constexpr int kWarps = 4 * STREAMS + STREAMS + 2, kThreads = 32 * kWarps;
+};
+constexpr int kMostSlots = 13, kAhead = 8;
+struct Bars {
+  uint64_t full[kMostSlots], free[kMostSlots];
+  uint64_t ready[kAhead];         // V blocks, by their number: the mending warp is never this many ahead of the products
+  uint64_t q_full[2], s_full[2][2], p_full[2][2], pv_done[2][2], drain[2];
+};
+}  // namespace tree_tc
+
+namespace tree {
+
+// The units of a CTA's piece, one after the other; every warp walks by itself
+template <int KB>
+struct Walk {
+  int b, h, length, cached, per_unit, j0, j1;
+  int64_t base, at, end, unit0;
+  // by a whole warp
+  __device__ void begin(const TreeParams& P, int lane, int group) {
+    int64_t total = 0;
+    Place p = {0, 0};
+    if (P.batch <= 32) {                  // one look at the lengths
+      const int64_t n = lane < P.batch ? ((int64_t)cache_blocks<KB>(P, lane) + draft_blocks<KB>(P)) * P.kv_heads : 0;
+      int64_t upto = n;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int64_t v = __shfl_up_sync(kFullMask, upto, o);
+        if (lane >= o) upto += v;
+      }
+      total = __shfl_sync(kFullMask, upto, 31);
+      at = piece_begin(total, group, P.groups);
+      const unsigned past = __ballot_sync(kFullMask, upto > at && lane < P.batch);
+      p.b = past ? __ffs(past) - 1 : P.batch;
+      p.base = __shfl_sync(kFullMask, upto - n, p.b & 31);
+    } else {
+      total = total_blocks<KB>(P, lane, P.batch);
+      at = piece_begin(total, group, P.groups);
+      p = place_of<KB>(P, lane, at);
+    }
+    end = piece_begin(total, group + 1, P.groups);
+    b = p.b;
+    base = p.base;
+  }
+  // the unit the piece is at, if it is not at its end
+  __device__ bool unit(const TreeParams& P) {
+    if (at >= end) return false;
+    length = length_of(P, b);
+    cached = (length + KB - 1) / KB;
+    per_unit = cached + draft_blocks<KB>(P);
+    h = (int)((at - base) / per_unit);
+    unit0 = base + (int64_t)h * per_unit;
+    j0 = (int)(at - unit0);
+    j1 = (int)min((int64_t)per_unit, end - unit0);
+    return true;
+  }
+  __device__ void next(const TreeParams& P) {
+    at = unit0 + j1;
+    if (at - base == (int64_t)per_unit * P.kv_heads) {
+      base = at;
+      ++b;
+    }
+  }
+};
+
+}  // namespace tree
+
+// Which of a cache's axes the coordinates move along (an axis of stride zero is one entry in its tensor map)
+struct TreeAxes { int kc_b, kc_h, vc_b, vc_h, k_b, k_h, v_b, v_h; };
+
+template <int D, int STREAMS, int SPLIT>
+__global__ void __launch_bounds__(tree_tc::Shape<D, STREAMS>::kThreads, 1)
+tree_tc_kernel(const __grid_constant__ CUtensorMap tmKc, const __grid_constant__ CUtensorMap tmVc, const __grid_constant__ CUtensorMap tmK,
+               const __grid_constant__ CUtensorMap tmV, const TreeParams P, const TreeAxes A, const int q_vec) {
+  using namespace ptx;
+  using namespace tree;
+  using namespace tree_tc;
+  using S = Shape<D, STREAMS>;
+  using Walker = Walk<kKeys>;
+  typedef __nv_bfloat16 T;
+  constexpr int NC = S::NC, kSlots = S::kSlots, LOOK = STREAMS == 1 ? 2 : 1, SOFT = 4 * STREAMS;
+  constexpr int RT = STREAMS * kRows / SPLIT;           // rows of the CTA's tile
+  constexpr int CW = kKeys / SPLIT;                     // keys of a thread in a block
+  constexpr uint32_t kTile = S::kTile, tO = STREAMS == 1 ? 256 : 128, tP0 = STREAMS == 1 ? 384 : 0;
+  extern __shared__ __align__(1024) uint8_t tree_tc_smem[];
+  __shared__ int abort_flag;
+  __shared__ uint32_t tmem_slot;
+  __shared__ __align__(8) Bars bars;
+  __shared__ volatile int odd_values[16];               // by unit: a drafted value is not finite
+  __shared__ float2 joined[SPLIT > 1 ? kRows : 1];      // maximum and sum of every copy of a row
+
+  const uint32_t sQ0 = smem_u32(tree_tc_smem), sRing = sQ0 + STREAMS * kTile;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int tile = blockIdx.x % P.tiles, group = blockIdx.x / P.tiles;
+  const int rows = P.tokens * P.G, row0 = tile * RT, here = min(RT, rows - row0);     // this tile's rows
+  const int streams = STREAMS == 2 && here > kRows ? 2 : 1;
+  // softmax warps with rows, of a stream
+  auto active = [&](int s) { return SPLIT > 1 ? 4 : max(0, min(4, (here - s * kRows + 31) / 32)); };
+
+  if (tid == 0) {
+    abort_flag = sQ0 & 1023u ? 1 : 0;                   // the tiles would be mis-swizzled: report instead of computing
+    for (int i = 0; i < kSlots; ++i) {
+      mbar_init(smem_u32(&bars.full[i]), 1);
+      mbar_init(smem_u32(&bars.free[i]), streams);
+    }
+    for (int i = 0; i < kAhead; ++i) mbar_init(smem_u32(&bars.ready[i]), 1);
+    for (int s = 0; s < streams; ++s) {
+      mbar_init(smem_u32(&bars.q_full[s]), 32 * active(s));
+      for (int i = 0; i < LOOK; ++i) {
+        mbar_init(smem_u32(&bars.s_full[s][i]), 1);
+        mbar_init(smem_u32(&bars.p_full[s][i]), 32 * active(s));
+        mbar_init(smem_u32(&bars.pv_done[s][i]), 1);
+      }
+      mbar_init(smem_u32(&bars.drain[s]), 1);
+    }
+    fence_mbar_init();
+    prefetch_tensormap(&tmKc);
+    prefetch_tensormap(&tmVc);
+    prefetch_tensormap(&tmK);
+    prefetch_tensormap(&tmV);
+  }
+  grid_allow_next();
+  Walker walk;
+  walk.begin(P, lane, group);
+  if (warp == 0) {
+    tmem_alloc(smem_u32(&tmem_slot), 512);
+    tmem_relinquish();
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  tc_fence_after_sync();
+  const uint32_t tm = tmem_slot;
+
+  if (warp < SOFT) {
+    // ------------------------------------------------------------------ softmax
+    const int s = warp >> 2, quarter = warp & 3;
+    const int part = quarter * SPLIT / 4;                                     // which keys of a block
+    const int lane_row = quarter * 32 + lane;                                 // row of the tensor-core tile
+    const int local = s * kRows + (SPLIT == 1 ? lane_row : lane_row % RT);    // row of the CTA's tile
+    const int row = row0 + local, t = row / P.G, g = row - t * P.G;
+    const bool valid = local < here;
+    const uint32_t tm_lane = tm + s * 256 + ((uint32_t)(quarter * 32) << 16);
+    const float scale2 = P.scale * kLog2e;
+    uint8_t* const region = tree_tc_smem + s * kTile;
+    auto stream_sync = [&]() { asm volatile("bar.sync %0, 128;" ::"r"(1 + s) : "memory"); };
+    const bool working = s < streams && (SPLIT > 1 || local - lane < here);
+    if (working && SPLIT > 1) {      // the keys that other copies take have weight zero here, always
+      float zero[16];
+#pragma unroll
+      for (int i = 0; i < 16; ++i) zero[i] = 0.f;
+#pragma unroll 1
+      for (int c = 0; c < 128; c += 16) tmem_st16(tm_lane + tP0 + c, zero);
+      tmem_st_wait();
+    }
+    uint32_t u = 0;
+    for (int seq = 0; working && walk.unit(P); walk.next(P), ++seq) {
+      // the query's row, swizzled as the products want it
+      {
+        const T* src = row_of<T>(P.q, walk.b, walk.h * P.G + g, t);
+#pragma unroll
+        for (int c = 0; c < D / 8; ++c) {
+          uint4 v = make_uint4(0, 0, 0, 0);
+          if (valid && c * 8 < P.d) {
+            if (q_vec) v = *reinterpret_cast<const uint4*>(src + c * 8);
+            else {
+              __align__(16) T x[8];
+#pragma unroll
+              for (int i = 0; i < 8; ++i) x[i] = src[c * 8 + i];
+              v = *reinterpret_cast<const uint4*>(x);
+            }
+          }
+          sts_v4(sQ0 + s * kTile + (c / 8) * 16384 + sw128_offset(lane_row, c & 7), v);
+        }
+        fence_proxy_async_smem();
+        mbar_arrive(smem_u32(&bars.q_full[s]));
+      }
+      float m_ref = -INFINITY, l = 0.f;
+      for (int j = walk.j0; j < walk.j1; ++j, ++u) {
+        const uint32_t buf = u % LOOK, phase = (u / LOOK) & 1;
+        const uint32_t tS = tm_lane + buf * 128;
+        const uint32_t tP = STREAMS == 1 ? tm_lane + tP0 + buf * 64 : tm_lane;
+        const bool draft = j >= walk.cached;
+        const int first = (draft ? j - walk.cached : j) * kKeys + part * CW, n = (draft ? P.tokens : walk.length) - first;
+        float x[CW / 32][32];
+        mbar_wait_warp(smem_u32(&bars.s_full[s][buf]), phase, &abort_flag);
+        tc_fence_after_sync();
+#pragma unroll
+        for (int k = 0; k < CW / 32; ++k) tmem_ld32(tS + part * CW + k * 32, x[k]);
+        tmem_ld_wait();
+        if (draft) {
+#pragma unroll
+          for (int k = 0; k < CW / 32; ++k) {
+            uint32_t seen = 0;
+            if (valid) {
+#pragma unroll 8
+              for (int i = 0; i < 32; ++i)
+                if (k * 32 + i < n && sees(P, walk.b, t, first + k * 32 + i)) seen |= 1u << i;
+            }
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              if (!(seen >> i & 1)) x[k][i] = -INFINITY;
+          }
+        } else if (n < CW) {
+#pragma unroll
+          for (int k = 0; k < CW / 32; ++k)
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              if (k * 32 + i >= n) x[k][i] = -INFINITY;
+        }
+        float m = max32(x[0]);
+#pragma unroll
+        for (int k = 1; k < CW / 32; ++k) m = fmaxf(m, max32(x[k]));
+        const float m2 = m * scale2;              // -inf: nothing seen
+        bool need = false;
+        float alpha = 1.f;
+        if (m_ref == -INFINITY) {
+          m_ref = m2;
+        } else if (m2 > m_ref + 8.f) {
+          alpha = ex2(m_ref - m2);
+          m_ref = m2;
+          l *= alpha;
+          need = true;
+        }
+        if (j > walk.j0 && __any_sync(kFullMask, need)) {
+          // with one S buffer the products of the block before are complete: S of this one came behind them
+          if (LOOK == 2) mbar_wait_warp(smem_u32(&bars.pv_done[s][(u - 1) % LOOK]), ((u - 1) / LOOK) & 1, &abort_flag);
+          tc_fence_after_sync();
+#pragma unroll 1
+          for (int c = 0; c < D; c += 16) {
+            float o[16];
+            tmem_ld16(tm_lane + tO + c, o);
+            tmem_ld_wait();
+#pragma unroll
+            for (int i = 0; i < 16; ++i) o[i] *= alpha;
+            tmem_st16(tm_lane + tO + c, o);
+          }
+          tmem_st_wait();
+        }
+        const float ref = m_ref == -INFINITY ? 0.f : m_ref;     // -inf - -inf must not be formed
+#pragma unroll
+        for (int k = 0; k < CW / 32; ++k) {
+          l += exp_row32(x[k], scale2, ref);
+          tmem_st_bf16_row32(tP + part * (CW / 2) + k * 16, x[k]);
+        }
+        tmem_st_wait();
+        tc_fence_before_sync();
+        mbar_arrive(smem_u32(&bars.p_full[s][buf]));
+      }
+      // the unit's end: O of this CTA's blocks, complete or a partial result
+      mbar_wait_warp(smem_u32(&bars.pv_done[s][(u - 1) % LOOK]), ((u - 1) / LOOK) & 1, &abort_flag);
+      tc_fence_after_sync();
+      const bool whole = walk.j0 == 0 && walk.j1 == walk.per_unit;
+      const int64_t slot = (int64_t)blockIdx.x * 2 + (walk.j0 == 0 ? 1 : 0);
+      const int u0 = max(0, walk.j0 - walk.cached) * kKeys, u1 = min(P.tokens, (walk.j1 - walk.cached) * kKeys);
+      const bool odd = odd_values[seq & 15] != 0;
+      // values that are not finite, of drafted rows that this row sees: columns c .. c + 7
+      auto add_odd = [&](int token, int c, float* o) {
+        for (int uu = u0; uu < u1; ++uu) {
+          if (!sees(P, walk.b, token, uu)) continue;
+          const T* v = row_of<T>(P.v, walk.b, walk.h, uu);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const float z = c + i < P.d ? __bfloat162float(v[c + i]) : 0.f;
+            if (!isfinite(z)) o[i] += z;
+          }
+        }
+      };
+      auto store8 = [&](int r, int token, int head, int c, float l_row, float* o) {       // columns c .. c + 7 of a row
+        if (odd) add_odd(token, c, o);
+        if (whole) {
+          if (c < P.d) {
+            const float inv = l_row > 0.f ? 1.f / l_row : (l_row == 0.f ? 0.f : l_row);      // a sum that is NaN stays NaN
+            uint4 v;
+            v.x = pack_bf16(o[0] * inv, o[1] * inv);
+            v.y = pack_bf16(o[2] * inv, o[3] * inv);
+            v.z = pack_bf16(o[4] * inv, o[5] * inv);
+            v.w = pack_bf16(o[6] * inv, o[7] * inv);
+            *reinterpret_cast<uint4*>(const_cast<T*>(row_of<T>(P.out, walk.b, head, token)) + c) = v;
+          }
+        } else {
+          float4* dst = reinterpret_cast<float4*>(P.partial + (slot * RT + r) * D + c);
+          dst[0] = make_float4(o[0], o[1], o[2], o[3]);
+          dst[1] = make_float4(o[4], o[5], o[6], o[7]);
+        }
+      };
+      auto store_stats = [&](int r, int token, int head, float m_row, float l_row) {
+        if (!whole) P.stats[slot * RT + r] = make_float2(m_row, l_row);
+        else if (P.lse != nullptr)
+          P.lse[((int64_t)walk.b * P.q_heads + head) * P.tokens + token] = l_row == 0.f ? -INFINITY : (m_row + log2f(l_row)) * kLn2;
+      };
+      if constexpr (SPLIT == 1) {
+#pragma unroll 1
+        for (int c = 0; c < D; c += 32) {
+          float o[32];
+          tmem_ld32(tm_lane + tO + c, o);
+          tmem_ld_wait();
+          if (valid)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) store8(local, t, walk.h * P.G + g, c + 8 * k, l, o + 8 * k);
+          __syncwarp();
+        }
+        if (valid) store_stats(local, t, walk.h * P.G + g, m_ref, l);
+      } else {
+        // join the copies: the upper half of them leaves its rows in Q's place, the lower half adds its own, then all threads
+        // take rows apart
+        joined[lane_row] = make_float2(m_ref, l);
+        stream_sync();
+        float top = -INFINITY, sum = 0.f;
+#pragma unroll
+        for (int k = 0; k < SPLIT; ++k) top = fmaxf(top, joined[k * RT + local].x);
+        const float base = top == -INFINITY ? 0.f : top;
+#pragma unroll
+        for (int k = 0; k < SPLIT; ++k) sum += joined[k * RT + local].y * ex2(joined[k * RT + local].x - base);
+        const float w = ex2(m_ref - base);
+        // row `local` of place k, 16-byte pieces exchanged against bank conflicts
+        auto piece = [&](int k, int r, int c4) { return reinterpret_cast<float4*>(region + (size_t)(k * RT + r) * (D * 4)) + (c4 ^ (r & 7)); };
+        if (part >= SPLIT / 2) {
+#pragma unroll 1
+          for (int c = 0; c < D; c += 16) {
+            float o[16];
+            tmem_ld16(tm_lane + tO + c, o);
+            tmem_ld_wait();
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              if (valid) *piece(part - SPLIT / 2, local, c / 4 + k) = make_float4(o[4 * k] * w, o[4 * k + 1] * w, o[4 * k + 2] * w, o[4 * k + 3] * w);
+          }
+        }
+        stream_sync();
+        if (part < SPLIT / 2) {
+#pragma unroll 1
+          for (int c = 0; c < D; c += 16) {
+            float o[16];
+            tmem_ld16(tm_lane + tO + c, o);
+            tmem_ld_wait();
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              if (!valid) continue;
+              float4* at = piece(part, local, c / 4 + k);
+              const float4 v = *at;
+              *at = make_float4(v.x + o[4 * k] * w, v.y + o[4 * k + 1] * w, v.z + o[4 * k + 2] * w, v.w + o[4 * k + 3] * w);
+            }
+          }
+        }
+        if (quarter == 0 || (SPLIT == 2 && quarter == 1)) {
+          if (valid) store_stats(local, t, walk.h * P.G + g, top, sum);
+        }
+        stream_sync();
+        for (int e = lane_row; e < here * (D / 8); e += 128) {
+          const int r = e / (D / 8), c = (e - r * (D / 8)) * 8, rr = row0 + r, token = rr / P.G;
+          float o[8], total = 0.f, high = -INFINITY;
+#pragma unroll
+          for (int k = 0; k < SPLIT; ++k) high = fmaxf(high, joined[k * RT + r].x);
+          const float low = high == -INFINITY ? 0.f : high;
+#pragma unroll
+          for (int k = 0; k < SPLIT; ++k) total += joined[k * RT + r].y * ex2(joined[k * RT + r].x - low);
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            float4 v = *piece(0, r, c / 4 + k);
+            if constexpr (SPLIT == 4) {
+              const float4 z = *piece(1, r, c / 4 + k);
+              v.x += z.x; v.y += z.y; v.z += z.z; v.w += z.w;
+            }
+            o[4 * k] = v.x; o[4 * k + 1] = v.y; o[4 * k + 2] = v.z; o[4 * k + 3] = v.w;
+          }
+          store8(r, token, walk.h * P.G + rr - token * P.G, c, total, o);
+        }
+        stream_sync();        // the rows have been read: Q of the next unit may take their place
+      }
+    }
+  } else if (warp < SOFT + STREAMS) {
+    // ------------------------------------------------------------------ MMA issuer of a stream
+    const int s = warp - SOFT;
+    if (s < streams) {
+      constexpr uint32_t idS = instr_desc_bf16(128, kKeys, false, false);
+      constexpr uint32_t idO = instr_desc_bf16(128, D, false, true);
+      const uint32_t ts = tm + s * 256;
+      const uint64_t dQ = smem_desc_sw128(sQ0 + s * kTile, 16);
+      uint32_t u = 0, su = 0, units = 0;      // blocks whose P V, whose S has been issued
+      auto issue_s = [&]() {
+        const uint32_t slot = 2 * su % kSlots, round = 2 * su / kSlots;
+        mbar_wait_bounded(smem_u32(&bars.full[slot]), round & 1, &abort_flag);
+        __syncwarp();
+        tc_fence_after_sync();
+        const uint64_t dK = smem_desc_sw128(sRing + slot * kTile, 16);
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k)
+          mma_bf16_elect(ts + (su % LOOK) * 128, desc_advance(dQ, (k / 4) * 16384 + (k % 4) * 32),
+                         desc_advance(dK, (k / 4) * 16384 + (k % 4) * 32), idS, k > 0);
+        mma_commit_elect(smem_u32(&bars.s_full[s][su % LOOK]));
+        mma_commit_elect(smem_u32(&bars.free[slot]));
+        ++su;
+      };
+      for (; walk.unit(P); walk.next(P), ++units) {
+        const int nb = walk.j1 - walk.j0;
+        mbar_wait_bounded(smem_u32(&bars.q_full[s]), units & 1, &abort_flag);
+        for (int t = 0; t < LOOK && t < nb; ++t) issue_s();
+        for (int t = 0; t < nb; ++t, ++u) {
+          const uint32_t slot = (2 * u + 1) % kSlots;
+          mbar_wait_bounded(smem_u32(&bars.ready[u % kAhead]), (u / kAhead) & 1, &abort_flag);
+          mbar_wait_bounded(smem_u32(&bars.p_full[s][u % LOOK]), (u / LOOK) & 1, &abort_flag);
+          __syncwarp();
+          tc_fence_after_sync();
+          const uint64_t dV = smem_desc_sw128(sRing + slot * kTile, 16384);
+          const uint32_t tP = STREAMS == 1 ? ts + tP0 + (u % LOOK) * 64 : ts;
+#pragma unroll
+          for (int k = 0; k < kKeys / 16; ++k) mma_bf16_tmem_a_elect(ts + tO, tP + k * 8, desc_advance(dV, k * 2048), idO, t > 0 || k > 0);
+          mma_commit_elect(smem_u32(&bars.pv_done[s][u % LOOK]));
+          mma_commit_elect(smem_u32(&bars.free[slot]));
+          if (t + LOOK < nb) issue_s();
+        }
+      }
+      // nothing of this CTA may still be running on the tensor cores when tensor memory is freed
+      mma_commit_elect(smem_u32(&bars.drain[s]));
+      mbar_wait_drain(smem_u32(&bars.drain[s]), 0);
+    }
+  } else if (warp == SOFT + STREAMS) {
+    // ------------------------------------------------------------------ TMA
+    uint32_t i = 0;
+    for (; walk.unit(P); walk.next(P)) {
+      for (int j = walk.j0; j < walk.j1; ++j) {
+        const bool draft = j >= walk.cached;
+        const int first = (draft ? j - walk.cached : j) * kKeys;
+#pragma unroll
+        for (int v = 0; v < 2; ++v, ++i) {
+          const uint32_t slot = i % kSlots, round = i / kSlots;
+          if (round >= 1) mbar_wait_bounded(smem_u32(&bars.free[slot]), (round - 1) & 1, &abort_flag);
+          if (lane == 0) {
+            const CUtensorMap* map = draft ? (v ? &tmV : &tmK) : (v ? &tmVc : &tmKc);
+            const int bb = walk.b * (draft ? (v ? A.v_b : A.k_b) : (v ? A.vc_b : A.kc_b));
+            const int hh = walk.h * (draft ? (v ? A.v_h : A.k_h) : (v ? A.vc_h : A.kc_h));
+            mbar_arrive_expect_tx(smem_u32(&bars.full[slot]), kTile);
+#pragma unroll
+            for (int c = 0; c < NC; ++c) tma_load_4d(sRing + slot * kTile + c * 16384, map, smem_u32(&bars.full[slot]), c * 64, first, hh, bb);
+          }
+          __syncwarp();
+        }
+      }
+    }
+    // every request must have landed before the block may exit (also when it gave up)
+    for (uint32_t back = 1; back <= (uint32_t)kSlots && back <= i; ++back)
+      mbar_wait_drain(smem_u32(&bars.full[(i - back) % kSlots]), ((i - back) / kSlots) & 1);
+  } else {
+    // ------------------------------------------------------------------ mending of V blocks
+    uint32_t u = 0;
+    for (int seq = 0; walk.unit(P); walk.next(P), ++seq) {
+      int odd = 0;
+      for (int j = walk.j0; j < walk.j1; ++j, ++u) {
+        const uint32_t slot = (2 * u + 1) % kSlots, round = (2 * u + 1) / kSlots;
+        const uint32_t at = sRing + slot * kTile;
+        // the K block as well: a slot that holds K and V in turn must not be asked about a phase before the one before it is over
+        mbar_wait_warp(smem_u32(&bars.full[2 * u % kSlots]), (2 * u / kSlots) & 1, &abort_flag);
+        mbar_wait_warp(smem_u32(&bars.full[slot]), round & 1, &abort_flag);
+        const bool draft = j >= walk.cached;
+        const int n = min(kKeys, (draft ? P.tokens - (j - walk.cached) * kKeys : walk.length - j * kKeys));
+        if (draft || n < kKeys) {
+          if (!draft)       // behind the drafted rows the tile is zero as loaded
+            for (int e = lane; e < (kKeys - n) * 8 * NC; e += 32)
+              sts_v4(at + (e & (NC - 1)) * 16384 + sw128_offset(n + (e / NC) / 8, (e / NC) & 7), make_uint4(0, 0, 0, 0));
+          else
+            for (int e = lane; e < n * 8 * NC; e += 32) {
+              const uint32_t p = at + (e & (NC - 1)) * 16384 + sw128_offset((e / NC) / 8, (e / NC) & 7);
+              const uint4 v = lds_v4(p);
+              uint32_t w[4] = {v.x, v.y, v.z, v.w};
+              bool bad = false;
+#pragma unroll
+              for (int k = 0; k < 4; ++k) {
+                if ((w[k] & 0x7f80u) == 0x7f80u) { w[k] &= 0xffff0000u; bad = true; }
+                if ((w[k] & 0x7f800000u) == 0x7f800000u) { w[k] &= 0xffffu; bad = true; }
+              }
+              if (bad) {
+                sts_v4(p, make_uint4(w[0], w[1], w[2], w[3]));
+                odd = 1;
+              }
+            }
+          fence_proxy_async_smem();
+          odd = __any_sync(kFullMask, odd);
+        }
+        if (lane == 0) {
+          if (j == walk.j1 - 1) odd_values[seq & 15] = odd;
+          mbar_arrive(smem_u32(&bars.ready[u % kAhead]));
+        }
+        __syncwarp();
+      }
+    }
+  }
+
+  tc_fence_before_sync();
+  __syncthreads();
+  if (warp == 0) tmem_dealloc(tm, 512);
+  if (tid == 0 && abort_flag && P.status != nullptr) atomicOr(P.status, 1);
+}
+
 // ---- joining the partial results -----------------------------------------------------------
 
 // A warp per row of a unit that more than one group of CTAs worked on
@@ -387,21 +902,39 @@ __global__ void __launch_bounds__(256) tree_merge_kernel(const TreeParams P) {
 
 struct TreePlan {
   bool tensor_cores;
-  int DP, RT, KB, ctas;      // padded dim_head, rows of a tile, keys of a block, CTAs the device holds at once
+  int DP, RT, KB, streams;   // padded dim_head, rows of a tile, keys of a block
   int tiles, groups;
   int64_t partial_bytes, bytes;
 };
 
+// Rows that TMA can fetch: 16-byte boundaries, strides the tiled format holds
+static bool tma_rows(const RowView& r, int64_t n) {
+  auto fits = [](int64_t s) { return s >= 0 && s % 8 == 0 && s < (1LL << 38); };
+  return (reinterpret_cast<uintptr_t>(r.p) & 15u) == 0 && fits(r.sb) && fits(r.sh) && fits(r.sn) && (r.sn > 0 || n <= 1);
+}
+
+static bool tc_serves(const TreeParams& P, int dtype) {
+  return dtype == NSA_BF16 && P.scale >= 1e-30f && P.scale <= 1e30f && tma_rows(P.k, P.tokens) && tma_rows(P.v, P.tokens) &&
+         (P.capacity == 0 || (tma_rows(P.kc, P.capacity) && tma_rows(P.vc, P.capacity))) &&
+         (reinterpret_cast<uintptr_t>(P.out.p) & 15u) == 0 && P.out.sb % 8 == 0 && P.out.sh % 8 == 0 && P.out.sn % 8 == 0;
+}
+
 static TreePlan plan_tree(const TreeParams& P, int dtype, int impl) {
-  (void)dtype; (void)impl;
   TreePlan p = {};
   const int64_t rows = (int64_t)P.tokens * P.G;
   p.DP = P.d <= 64 ? 64 : 128;
-  p.RT = rows <= 8 ? 8 : 32;
-  p.KB = tree_simt::kKeys;
-  p.ctas = 2 * 148;
+  p.tensor_cores = impl != NSA_IMPL_SIMT && tc_serves(P, dtype);
+  int64_t ctas = num_sms();
+  if (p.tensor_cores) {
+    p.RT = rows <= 32 ? 32 : rows <= 64 ? 64 : rows <= 128 ? 128 : 256;
+    p.KB = tree_tc::kKeys;
+  } else {
+    p.RT = rows <= 8 ? 8 : 32;
+    p.KB = tree_simt::kKeys;
+    ctas *= 2;
+  }
   p.tiles = (int)((rows + p.RT - 1) / p.RT);
-  p.groups = p.tiles >= p.ctas ? 1 : p.ctas / p.tiles;
+  p.groups = p.tiles >= ctas ? 1 : (int)(ctas / p.tiles);
   // no more groups than there can be blocks
   const int64_t most = (int64_t)P.batch * P.kv_heads * (((int64_t)P.capacity + p.KB - 1) / p.KB + (P.tokens + p.KB - 1) / p.KB);
   if (p.groups > most) p.groups = (int)most;
@@ -411,8 +944,32 @@ static TreePlan plan_tree(const TreeParams& P, int dtype, int impl) {
   return p;
 }
 
-int64_t tree_workspace_bytes(const TreeParams& P, int dtype, int impl) {
-  return plan_tree(P, dtype, impl).bytes;
+int64_t tree_workspace_bytes(const TreeParams& P, int dtype, int impl) { return plan_tree(P, dtype, impl).bytes; }
+
+#define TREE_TRY(expr)                                                        \
+  do {                                                                        \
+    const cudaError_t e_ = (expr);                                            \
+    if (e_ != cudaSuccess) return fail((int)e_, cudaGetErrorString(e_));     \
+  } while (0)
+
+// The merge starts while the last CTAs of the kernel before it are still at work, and waits for their results
+template <typename T, int DP, int RT, int KB>
+static int run_merge(const TreeParams& P, const TreePlan& p, cudaStream_t stream) {
+  if (p.groups > 1) {
+    cudaLaunchConfig_t config = {};
+    config.gridDim = dim3((unsigned)(((int64_t)P.tokens * P.G + 7) / 8), (unsigned)(P.batch * P.kv_heads));
+    config.blockDim = dim3(256);
+    config.stream = stream;
+    cudaLaunchAttribute overlap = {};
+    overlap.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    overlap.val.programmaticStreamSerializationAllowed = 1;
+    config.attrs = &overlap;
+    config.numAttrs = 1;
+    TREE_TRY(cudaLaunchKernelEx(&config, tree_merge_kernel<T, DP, RT, KB>, P));
+  }
+  TREE_TRY(cudaGetLastError());
+  count_launches(p.groups > 1 ? 2 : 1);
+  return NSA_OK;
 }
 
 template <typename T, int DP, int RT>
@@ -421,16 +978,9 @@ static int run_simt(const TreeParams& P, const TreePlan& p, cudaStream_t stream)
   auto wide = [](const RowView& r) { return (reinterpret_cast<uintptr_t>(r.p) & 15u) == 0 && r.sb % V == 0 && r.sh % V == 0 && r.sn % V == 0; };
   const int vec = wide(P.k) && wide(P.v) && (P.capacity == 0 || (wide(P.kc) && wide(P.vc)));
   const int smem = tree_simt::Shape<DP, RT>::kFloats * (int)sizeof(float);
-  cudaError_t err = allow_shared_memory<tree_simt_kernel<T, DP, RT>>();
-  if (err != cudaSuccess) return fail((int)err, cudaGetErrorString(err));
+  TREE_TRY((allow_shared_memory<tree_simt_kernel<T, DP, RT>>()));
   tree_simt_kernel<T, DP, RT><<<(unsigned)(p.groups * p.tiles), tree_simt::kThreads, smem, stream>>>(P, vec);
-  if (p.groups > 1) {
-    const dim3 grid((unsigned)(((int64_t)P.tokens * P.G + 7) / 8), (unsigned)(P.batch * P.kv_heads));
-    tree_merge_kernel<T, DP, RT, tree_simt::kKeys><<<grid, 256, 0, stream>>>(P);
-  }
-  count_launches(p.groups > 1 ? 2 : 1);
-  err = cudaGetLastError();
-  return err == cudaSuccess ? NSA_OK : fail((int)err, cudaGetErrorString(err));
+  return run_merge<T, DP, RT, tree_simt::kKeys>(P, p, stream);
 }
 
 template <typename T>
@@ -439,14 +989,51 @@ static int run_simt_typed(const TreeParams& P, const TreePlan& p, cudaStream_t s
   return p.RT == 8 ? run_simt<T, 128, 8>(P, p, stream) : run_simt<T, 128, 32>(P, p, stream);
 }
 
+// Boxes of 64 features x 128 rows of one head.  An axis of one entry, or of stride zero, is one entry in the map; `step_b` and
+// `step_h` say whether coordinates move along it.
+static int make_tree_map(CUtensorMap* map, const RowView& r, int B, int H, int64_t N, int d, int* step_b, int* step_h) {
+  *step_b = B > 1 && r.sb > 0;
+  *step_h = H > 1 && r.sh > 0;
+  const uint64_t row = N > 1 ? (uint64_t)r.sn * 2 : (uint64_t)d * 2;
+  const uint64_t dims[4] = {(uint64_t)d, (uint64_t)N, (uint64_t)(*step_h ? H : 1), (uint64_t)(*step_b ? B : 1)};
+  const uint64_t strides[3] = {row, *step_h ? (uint64_t)r.sh * 2 : row, *step_b ? (uint64_t)r.sb * 2 : row};
+  const uint32_t box[4] = {64, tree_tc::kKeys, 1, 1};
+  return encode_bf16_tiles(map, r.p, dims, strides, box);
+}
+
+template <int D, int STREAMS, int SPLIT>
+static int run_tc(const TreeParams& P, const TreePlan& p, cudaStream_t stream) {
+  using S = tree_tc::Shape<D, STREAMS>;
+  CUtensorMap tmKc, tmVc, tmK, tmV;
+  TreeAxes A = {};
+  int rc = make_tree_map(&tmK, P.k, P.batch, P.kv_heads, P.tokens, P.d, &A.k_b, &A.k_h);
+  if (rc == NSA_OK) rc = make_tree_map(&tmV, P.v, P.batch, P.kv_heads, P.tokens, P.d, &A.v_b, &A.v_h);
+  tmKc = tmK; tmVc = tmV;                 // an empty cache is never looked at
+  if (rc == NSA_OK && P.capacity > 0) rc = make_tree_map(&tmKc, P.kc, P.batch, P.kv_heads, P.capacity, P.d, &A.kc_b, &A.kc_h);
+  if (rc == NSA_OK && P.capacity > 0) rc = make_tree_map(&tmVc, P.vc, P.batch, P.kv_heads, P.capacity, P.d, &A.vc_b, &A.vc_h);
+  if (rc != NSA_OK) return rc;
+  const int q_vec = (reinterpret_cast<uintptr_t>(P.q.p) & 15u) == 0 && P.q.sb % 8 == 0 && P.q.sh % 8 == 0 && P.q.sn % 8 == 0;
+  TREE_TRY((allow_shared_memory<tree_tc_kernel<D, STREAMS, SPLIT>>()));
+  tree_tc_kernel<D, STREAMS, SPLIT><<<(unsigned)(p.groups * p.tiles), S::kThreads, S::kBytes, stream>>>(tmKc, tmVc, tmK, tmV, P, A, q_vec);
+  return run_merge<__nv_bfloat16, D, STREAMS * tree_tc::kRows / SPLIT, tree_tc::kKeys>(P, p, stream);
+}
+
+template <int D>
+static int run_tc_rows(const TreeParams& P, const TreePlan& p, cudaStream_t stream) {
+  if (p.RT == 32) return run_tc<D, 1, 4>(P, p, stream);
+  if (p.RT == 64) return run_tc<D, 1, 2>(P, p, stream);
+  return p.RT == 128 ? run_tc<D, 1, 1>(P, p, stream) : run_tc<D, 2, 1>(P, p, stream);
+}
+
 int launch_tree(TreeParams& P, int dtype, int impl, uint8_t* workspace, cudaStream_t stream) {
   const TreePlan p = plan_tree(P, dtype, impl);
-  if (impl == NSA_IMPL_SM100) return fail(NSA_ERR_UNSUPPORTED, "tree: not served by the tensor-core kernel");
+  if (impl == NSA_IMPL_SM100 && !p.tensor_cores) return fail(NSA_ERR_UNSUPPORTED, "tree: not served by the tensor-core kernel");
   if ((int64_t)p.groups * p.tiles > 0x7fffffffLL || (int64_t)P.batch * P.kv_heads > 65535)
     return fail(NSA_ERR_SHAPE, "tree: too many rows, or more than 65535 KV heads over the batch");
   P.tiles = p.tiles; P.groups = p.groups;
   P.partial = reinterpret_cast<float*>(workspace);
   P.stats = reinterpret_cast<float2*>(workspace + p.partial_bytes);
+  if (p.tensor_cores) return p.DP == 64 ? run_tc_rows<64>(P, p, stream) : run_tc_rows<128>(P, p, stream);
   return dtype == NSA_F32 ? run_simt_typed<float>(P, p, stream) : run_simt_typed<__nv_bfloat16>(P, p, stream);
 }
 
