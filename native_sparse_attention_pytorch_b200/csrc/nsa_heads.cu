@@ -5,13 +5,13 @@
 //
 // Angles.  A frequency is held as a 64-bit fraction of a turn per position, so position times frequency is an integer
 // product whose overflow drops whole turns: the phase is exact to pos * 2^-65 turns, where a product in fp32 is off by 0.03
-// radians at position 10^6.  Its upper 32 bits, as fp32 in [-1, 1) half turns, go to sincospif: 10^-7 in the end.
+// radians at position 10^6.  Sines and cosines of it are good to 10^-7 at any position.
 // Angles are formed in the kernel: one set per token serves all its heads, so there is no table to build, keep or read.
 //
-// Work.  A row (one head of one token) belongs to 2^k neighbouring lanes, a lane to `units` of two vectors of W elements:
-// with the half layout the two vectors whose elements form pairs, else two neighbouring vectors.  A group of lanes goes
-// through up to `per_slot` heads of a token (a slot: heads of the queries or of the keys), kBatch of them in flight.
-// What bounds it is the traffic: x (and dy) in, y (or dx) out.
+// Work.  A row (one head of one token) belongs to 2^k neighbouring lanes, a lane to `units` of two vectors of W elements, whose
+// elements are W pairs (u, v): with the half layout u from one vector and v from the other, else even and odd elements of both.
+// A group of lanes goes through up to `per_slot` heads of a token (a slot: heads of the queries or of the keys), kBatch of them in
+// flight.  What bounds it is the traffic: x (and dy) in, y (or dx) out.
 
 #include "nsa_common.cuh"
 #include "nsa_kernels.h"
@@ -19,9 +19,21 @@
 
 namespace nsa {
 
+#ifndef HEADS_MB
+#define HEADS_MB 4
+#define HEADS_HN 1
+#define HEADS_HB 4
+#define HEADS_PER 32
+#define HEADS_W 6
+#define HEADS_R 4
+#endif
 namespace heads {
 
-constexpr int kThreads = 256;
+#ifndef HEADS_T
+#define HEADS_T 128
+#endif
+constexpr int kThreads = HEADS_T;
+enum { kNone = 0, kShared = 1, kPerHead = 2 };
 
 template <int BYTES> struct RawOf;
 template <> struct RawOf<16> { typedef uint4 type; };
@@ -47,195 +59,302 @@ struct Vec {
   }
 };
 
-// Where a unit's two vectors lie in the row (-1: not there), and which of its W pairs are rotated by which frequencies
+// Where a unit's two vectors lie in the row (-1: not there), the frequencies of their first pairs, and whether they are rotated
 struct Unit {
-  int a, b;        // first elements
-  int freq;        // frequency of the first pair
-  int pairs;       // rotated pairs
+  int a, b, freq_a, freq_b;
+  bool rot_a, rot_b;
 };
 
-template <int W>
+template <int W, bool HALF>
 __device__ __forceinline__ Unit unit_at(const HeadsParams& P, int u) {
   Unit t;
-  if (P.half) {
+  if (HALF) {
     const int rot = P.rotary_dim / 2 / W;
-    if (u < rot) {
-      t.a = u * W; t.b = P.rotary_dim / 2 + u * W; t.freq = u * W; t.pairs = W;
-      return t;
-    }
-    t.a = P.rotary_dim + 2 * (u - rot) * W; t.freq = 0; t.pairs = 0;
-  } else {
-    t.a = 2 * u * W; t.freq = u * W;
-    t.pairs = max(0, min(W, P.rotary_dim / 2 - u * W));
+    t.rot_a = t.rot_b = u < rot;
+    t.a = u < rot ? u * W : P.rotary_dim + 2 * (u - rot) * W;
+    t.b = u < rot ? P.rotary_dim / 2 + u * W : t.a + W;
+    t.freq_a = t.freq_b = u * W;
+  } else if (W == 1) {
+    t.a = 2 * u; t.b = 2 * u + 1;
+    t.freq_a = t.freq_b = u;
+    t.rot_a = t.rot_b = 2 * u < P.rotary_dim;
+  } else {             // neighbouring lanes take neighbouring vectors
+    t.a = u * W;
+    t.b = t.a + (P.d / W + 1) / 2 * W;
+    if (t.a >= (P.d / W + 1) / 2 * W) t.a = t.b = P.d;
+    t.freq_a = t.a / 2; t.freq_b = t.b / 2;
+    t.rot_a = t.a < P.rotary_dim; t.rot_b = t.b < P.rotary_dim;
   }
-  t.b = t.a + W < P.d ? t.a + W : -1;
-  if (t.a >= P.d) t.a = -1;
+  if (t.a >= P.d) { t.a = -1; t.rot_a = false; }
+  if (t.b >= P.d) { t.b = -1; t.rot_b = HALF && t.rot_a; }
   return t;
 }
 
-// The rotation of a unit's values, a and b; sine negated for the way back
-template <int W>
-__device__ __forceinline__ void turn(bool half, int pairs, const float* co, const float* si, float* a, float* b) {
+// The first pairs of a unit lie in its first vector (half layout: all of them in both)
+template <int W, bool HALF>
+__host__ __device__ constexpr int first_pairs() { return HALF || W == 1 ? W : W / 2; }
+
+template <typename T, int W, bool HALF>
+__device__ __forceinline__ void split(const typename Vec<T, W>::Raw& a, const typename Vec<T, W>::Raw& b, float* u, float* v) {
+  float x[W], y[W];
+  Vec<T, W>::widen(a, x);
+  Vec<T, W>::widen(b, y);
 #pragma unroll
   for (int i = 0; i < W; ++i) {
-    // half (and single elements): a[i] with b[i]; else neighbours inside the 2 W elements of a, b
-    float* x = (half || W == 1) ? a + i : (2 * i < W ? a + 2 * i : b + 2 * i - W);
-    float* z = (half || W == 1) ? b + i : x + 1;
-    if (i < pairs) {
-      const float x0 = *x, z0 = *z;
-      *x = x0 * co[i] - z0 * si[i];
-      *z = z0 * co[i] + x0 * si[i];
+    if (HALF || W == 1) {
+      u[i] = x[i]; v[i] = y[i];
+    } else {
+      u[i] = 2 * i < W ? x[(2 * i) % W] : y[(2 * i) % W];
+      v[i] = 2 * i < W ? x[(2 * i + 1) % W] : y[(2 * i + 1) % W];
     }
   }
+}
+// A unit's weights, of head h where there is a row per head
+template <typename T, int W, bool HALF>
+__device__ __forceinline__ void load_weight(const HeadsParams& P, const HeadRows& R, const Unit& t, int h, float* wu, float* wv) {
+  const int64_t row = P.weight_per_head ? (int64_t)h * P.d : 0;
+  auto weight = [&](int e) { return P.weight_f32 ? __ldg((const float*)R.weight + row + e) : Elem<T>::to_float(((const T*)R.weight)[row + e]); };
+#pragma unroll
+  for (int i = 0; i < W; ++i) {
+    const bool second = !HALF && W > 1 && 2 * i >= W;
+    const int at = HALF || W == 1 ? t.a : (second ? t.b : t.a);
+    const int eu = HALF || W == 1 ? t.a + i : at + (2 * i) % W, ev = HALF || W == 1 ? t.b + i : eu + 1;
+    wu[i] = at < 0 ? 0.f : weight(eu);
+    wv[i] = (HALF || W == 1 ? t.b : at) < 0 ? 0.f : weight(ev);
+  }
+}
+template <typename T, int W, bool HALF, bool FULL>
+__device__ __forceinline__ void store(const Unit& t, T* row, const float* u, const float* v) {
+  float x[W], y[W];
+#pragma unroll
+  for (int i = 0; i < W; ++i) {
+    if (HALF || W == 1) {
+      x[i] = u[i]; y[i] = v[i];
+    } else if (2 * i < W) {
+      x[(2 * i) % W] = u[i]; x[(2 * i + 1) % W] = v[i];
+    } else {
+      y[(2 * i) % W] = u[i]; y[(2 * i + 1) % W] = v[i];
+    }
+  }
+  if (FULL || t.a >= 0) Vec<T, W>::store(row + t.a, x);
+  if (FULL || t.b >= 0) Vec<T, W>::store(row + t.b, y);
+}
+
+// (u, v) -> (u cu - v cv, v dv + u du): N pairs
+template <int N>
+__device__ __forceinline__ void rotate(float* u, float* v, const float* cu, const float* cv, const float* dv, const float* du) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const float a = u[i] * cu[i] - v[i] * cv[i];
+    v[i] = v[i] * dv[i] + u[i] * du[i];
+    u[i] = a;
+  }
+}
+
+// Sine and cosine of a phase, 2^64 to the turn.  The nearest quarter turn is taken off in integers; what is left, at most pi / 4, goes
+// into the Taylor series up to x^9 and x^8, whose next terms are below 2e-9 and 2.5e-8 (half a unit of a cosine above 0.7 is 3e-8).
+// Its 30 bits as fp32 are off by 2^-25 of pi / 4 at most.
+__device__ __forceinline__ void sine_cosine(uint64_t phase, float& si, float& co) {
+  const uint32_t top = (uint32_t)((phase + 0x80000000ull) >> 32), quarter = (top + 0x20000000u) >> 30;
+  const float x = (float)(int32_t)(top - (quarter << 30)) * 1.4629180792671596e-9f;      // 2 pi / 2^32
+  const float y = x * x;
+  const float s = x + x * y * (-1.f / 6 + y * (1.f / 120 + y * (-1.f / 5040 + y * (1.f / 362880))));
+  const float c = 1.f + y * (-0.5f + y * (1.f / 24 + y * (-1.f / 720 + y * (1.f / 40320))));
+  si = __uint_as_float(__float_as_uint(quarter & 1 ? c : s) ^ (quarter & 2) << 30);
+  co = __uint_as_float(__float_as_uint(quarter & 1 ? s : c) ^ ((quarter + 1) & 2) << 30);
+}
+
+// Sum over the lanes of a row
+__device__ __forceinline__ float row_sum(float v, int lanes) {
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1)
+    if (o < lanes) v += __shfl_xor_sync(kFullMask, v, o);
+  return v;
 }
 
 }  // namespace heads
 
 // W: elements of a vector; UPL: units of a lane; HALF: the layout
-template <typename T, int W, int UPL, bool HALF, bool NORM, bool BWD>
-__global__ void __launch_bounds__(heads::kThreads, 2) heads_kernel(const HeadsParams P) {
+// WEIGHTS: kNone (no norm), kShared, kPerHead
+// FULL: every lane has both vectors of every unit
+template <typename T, int W, int UPL, bool HALF, int WEIGHTS, bool BWD, bool FULL>
+__global__ void __launch_bounds__(heads::kThreads, HEADS_MB) heads_kernel(const HeadsParams P) {
   using namespace heads;
   using V = Vec<T, W>;
   typedef typename V::Raw Raw;
-  constexpr bool XIN = !BWD || NORM;                 // x is read
-  constexpr int kBatch = UPL > 1 ? 1 : (BWD && NORM ? 2 : 4);   // heads in flight
+  constexpr bool NORM = WEIGHTS != kNone;
+  constexpr bool XIN = !BWD || NORM;                              // x is read
+  constexpr bool FOLD = WEIGHTS == kShared && !BWD;               // the weights are part of the rotation's factors
+  constexpr bool ONE = WEIGHTS == kPerHead && BWD;                // one head a slot, whose weight gradient stays in registers
+  constexpr int kBatch = UPL > 1 || ONE ? 1 : (BWD && NORM ? HEADS_HN : HEADS_HB);     // heads in flight
+  constexpr int FIRST = first_pairs<W, HALF>();
   __shared__ float fold[NORM && BWD ? kThreads / 32 : 1][NORM && BWD ? kHeadsMaxDim : 1];
+  __shared__ __align__(16) float held[NORM && BWD ? 32 * UPL : 1][NORM && BWD ? 2 * W : 1];   // the backward's weights, unit by unit
 
+  ptx::grid_allow_next();
   const int lanes = 1 << P.lane_shift, lane = threadIdx.x & (lanes - 1);
   const int group = threadIdx.x >> P.lane_shift, groups = kThreads >> P.lane_shift;
-  const bool keys = (int)blockIdx.y >= P.slots[0];
+  // blocks of the queries' slots, then of the keys'
+  const bool keys = (int)blockIdx.x >= P.slots[0] * P.blocks[0];
   const HeadRows& R = P.part[keys];
-  const int slot = (int)blockIdx.y - (keys ? P.slots[0] : 0);
+  const int block = (int)blockIdx.x - (keys ? P.slots[0] * P.blocks[0] : 0), blocks = P.blocks[keys];
+  const int slot = block / blocks, at_block = block - slot * blocks;
   const int h0 = slot * P.per_slot, h1 = min(R.heads, h0 + P.per_slot);
 
   Unit unit[UPL];
-  float w[UPL][2 * W], acc[UPL][2 * W];
+  float wu[FOLD ? UPL : 1][W], wv[FOLD ? UPL : 1][W], acc_u[UPL][W], acc_v[UPL][W];
 #pragma unroll
   for (int k = 0; k < UPL; ++k) {
-    unit[k] = unit_at<W>(P, lane + k * lanes);
-    if (NORM) {
-      const int64_t row = P.weight_per_head ? (int64_t)h0 * P.d : 0;    // per head: one head a slot
+    unit[k] = unit_at<W, HALF>(P, lane + k * lanes);
+    if (FOLD) load_weight<T, W, HALF>(P, R, unit[k], 0, wu[FOLD ? k : 0], wv[FOLD ? k : 0]);
+    if (NORM && BWD) {
+      if (group == 0) load_weight<T, W, HALF>(P, R, unit[k], h0, held[lane + k * lanes], held[lane + k * lanes] + W);
 #pragma unroll
-      for (int i = 0; i < W; ++i) {
-        const int ea = unit[k].a + i, eb = unit[k].b + i;
-        w[k][i] = unit[k].a < 0 ? 0.f : P.weight_f32 ? ((const float*)R.weight)[row + ea] : Elem<T>::to_float(((const T*)R.weight)[row + ea]);
-        w[k][W + i] = unit[k].b < 0 ? 0.f : P.weight_f32 ? ((const float*)R.weight)[row + eb] : Elem<T>::to_float(((const T*)R.weight)[row + eb]);
-        acc[k][i] = acc[k][W + i] = 0.f;
-      }
+      for (int i = 0; i < W; ++i) acc_u[k][i] = acc_v[k][i] = 0.f;
     }
   }
+  if (NORM && BWD) __syncthreads();
 
   const unsigned tokens = (unsigned)P.batch * (unsigned)P.seq;
   const float inv_d = 1.f / (float)P.d;
   // every lane of a warp takes part in the sums over a row: groups without a token go along with nothing to load
-  for (unsigned first = blockIdx.x * groups; first < tokens; first += gridDim.x * groups) {
+  for (unsigned first = at_block * groups; first < tokens; first += blocks * groups) {
     const unsigned token = first + group;
     const bool live = token < tokens;
     const unsigned b = live ? token / (unsigned)P.seq : 0, n = live ? token - b * (unsigned)P.seq : 0;
+    const T* xp = XIN ? (const T*)R.x + (int64_t)b * R.x_sb + (int64_t)n * R.x_sn + (int64_t)h0 * R.x_sh : nullptr;
+    const T* gp = BWD ? (const T*)R.dy + (int64_t)b * R.dy_sb + (int64_t)n * R.dy_sn + (int64_t)h0 * R.dy_sh : nullptr;
+    T* op = (T*)R.out + (int64_t)b * R.o_sb + (int64_t)n * R.o_sn + (int64_t)h0 * R.o_sh;
+    Raw xr[kBatch][UPL][2], gr[BWD ? kBatch : 1][UPL][2];
+    // the next head's values into place j; beyond the slot's heads (and, with FULL, for groups without a token) those of the last
+    // one, of which nothing is kept
+    int ahead = h0;
+    auto fetch = [&](int j) {
+#pragma unroll
+      for (int k = 0; k < UPL; ++k) {
+        const bool a = FULL || (live && unit[k].a >= 0), b = FULL || (live && unit[k].b >= 0);
+        if (XIN) {
+          xr[j][k][0] = a ? V::load(xp + unit[k].a) : Raw{};
+          xr[j][k][1] = b ? V::load(xp + unit[k].b) : Raw{};
+        }
+        if (BWD) {
+          gr[j][k][0] = a ? V::load(gp + unit[k].a) : Raw{};
+          gr[j][k][1] = b ? V::load(gp + unit[k].b) : Raw{};
+        }
+      }
+      if (++ahead < h1) {
+        if (XIN) xp += R.x_sh;
+        if (BWD) gp += R.dy_sh;
+      }
+    };
+#pragma unroll
+    for (int j = 0; j < kBatch; ++j) fetch(j);                 // under way while the angles are formed
     int64_t pos = P.offset + n;
     if (P.positions != nullptr) {
       const int64_t at = (int64_t)b * P.pos_sb + n;
       pos = P.offset + (P.pos_i64 ? ((const int64_t*)P.positions)[at] : (int64_t)((const int32_t*)P.positions)[at]);
     }
-    float co[UPL][W], si[UPL][W];
+    // factors of the rotation: u' = u cu - v cv, v' = v dv + u du; with the weights in them (FOLD), else two sets are enough
+    float cu[UPL][W], cv[UPL][W], dv[FOLD ? UPL : 1][W], du[FOLD ? UPL : 1][W];
 #pragma unroll
     for (int k = 0; k < UPL; ++k)
 #pragma unroll
       for (int i = 0; i < W; ++i) {
-        co[k][i] = 1.f; si[k][i] = 0.f;
-        if (i < unit[k].pairs) {
-          const uint64_t phase = (uint64_t)pos * __ldg(P.steps + unit[k].freq + i);
-          const int32_t top = (int32_t)((phase + 0x80000000ull) >> 32);
-          sincospif((float)top * 4.656612873077393e-10f, &si[k][i], &co[k][i]);    // 2^-31: a turn is two half turns
-          co[k][i] *= P.magnitude;
-          si[k][i] *= BWD ? -P.magnitude : P.magnitude;
+        float co = 1.f, si = 0.f;
+        if (i < FIRST ? unit[k].rot_a : unit[k].rot_b) {
+          sine_cosine((uint64_t)pos * __ldg(P.steps + (i < FIRST ? unit[k].freq_a + i : unit[k].freq_b + i - FIRST)), si, co);
+          co *= P.magnitude;
+          si *= BWD ? -P.magnitude : P.magnitude;
+        }
+        cu[k][i] = co; cv[k][i] = si;
+        if (FOLD) {
+          const int f = FOLD ? k : 0;
+          dv[f][i] = wv[f][i] * co; du[f][i] = wu[f][i] * si;
+          cu[k][i] *= wu[f][i]; cv[k][i] *= wv[f][i];
         }
       }
-    const T* xp = XIN ? (const T*)R.x + (int64_t)b * R.x_sb + (int64_t)n * R.x_sn : nullptr;
-    const T* gp = BWD ? (const T*)R.dy + (int64_t)b * R.dy_sb + (int64_t)n * R.dy_sn : nullptr;
-    T* op = (T*)R.out + (int64_t)b * R.o_sb + (int64_t)n * R.o_sn;
     for (int h = h0; h < h1; h += kBatch) {
-      Raw xr[kBatch][UPL][2], gr[BWD ? kBatch : 1][UPL][2];
-#pragma unroll
-      for (int j = 0; j < kBatch; ++j)
-#pragma unroll
-        for (int k = 0; k < UPL; ++k) {
-          const bool ok = live && h + j < h1;
-          if (XIN) {
-            xr[j][k][0] = ok && unit[k].a >= 0 ? V::load(xp + (h + j) * R.x_sh + unit[k].a) : Raw{};
-            xr[j][k][1] = ok && unit[k].b >= 0 ? V::load(xp + (h + j) * R.x_sh + unit[k].b) : Raw{};
-          }
-          if (BWD) {
-            gr[j][k][0] = ok && unit[k].a >= 0 ? V::load(gp + (h + j) * R.dy_sh + unit[k].a) : Raw{};
-            gr[j][k][1] = ok && unit[k].b >= 0 ? V::load(gp + (h + j) * R.dy_sh + unit[k].b) : Raw{};
-          }
-        }
 #pragma unroll
       for (int j = 0; j < kBatch; ++j) {
         const bool ok = live && h + j < h1;
-        float x[UPL][2 * W], g[UPL][2 * W];
-        float rstd = 1.f, c = 0.f;
-        if (NORM) {
-          float ss = 0.f;
+        float u[UPL][W], v[UPL][W], gu[BWD ? UPL : 1][W], gv[BWD ? UPL : 1][W];          // x, dy; then what is stored
 #pragma unroll
-          for (int k = 0; k < UPL; ++k) {
-            V::widen(xr[j][k][0], x[k]);
-            V::widen(xr[j][k][1], x[k] + W);
-#pragma unroll
-            for (int i = 0; i < 2 * W; ++i) ss += x[k][i] * x[k][i];
-          }
-          for (int o = lanes >> 1; o > 0; o >>= 1) ss += __shfl_xor_sync(kFullMask, ss, o);
-          rstd = rsqrtf(ss * inv_d + P.eps);
-        } else if (!BWD) {
-#pragma unroll
-          for (int k = 0; k < UPL; ++k) {
-            V::widen(xr[j][k][0], x[k]);
-            V::widen(xr[j][k][1], x[k] + W);
-          }
+        for (int k = 0; k < UPL; ++k) {
+          if (XIN) split<T, W, HALF>(xr[j][k][0], xr[j][k][1], u[k], v[k]);
+          if (BWD) split<T, W, HALF>(gr[j][k][0], gr[j][k][1], gu[k], gv[k]);
         }
-        if (BWD) {
-          float dot = 0.f;
+        if (!ONE) fetch(j);                  // the place is free: the next head's values are on their way meanwhile
+        float rstd = 1.f;
+        if (NORM) {
+          float ss = 0.f, st = 0.f;
+#pragma unroll
+          for (int k = 0; k < UPL; ++k)
+#pragma unroll
+            for (int i = 0; i < W; ++i) { ss += u[k][i] * u[k][i]; st += v[k][i] * v[k][i]; }
+          rstd = rsqrtf(row_sum(ss + st, lanes) * inv_d + P.eps);
+#pragma unroll
+          for (int k = 0; k < UPL; ++k)
+#pragma unroll
+            for (int i = 0; i < W; ++i) { u[k][i] *= rstd; v[k][i] *= rstd; }
+        }
+        auto turn = [&](int k, float* p, float* q) {
+          const float* d = FOLD ? dv[FOLD ? k : 0] : cu[k];
+          const float* e = FOLD ? du[FOLD ? k : 0] : cv[k];
+          if (unit[k].rot_a && unit[k].rot_b) rotate<W>(p, q, cu[k], cv[k], d, e);
+          else {                             // a pair that is not rotated must not be multiplied with the other's zero
+            if (unit[k].rot_a) rotate<FIRST>(p, q, cu[k], cv[k], d, e);
+            if (unit[k].rot_b && FIRST < W) rotate<W - FIRST>(p + FIRST, q + FIRST, cu[k] + FIRST, cv[k] + FIRST, d + FIRST, e + FIRST);
+            if (FOLD)
+#pragma unroll
+              for (int i = 0; i < W; ++i)
+                if (!(i < FIRST ? unit[k].rot_a : unit[k].rot_b)) { p[i] *= cu[k][i]; q[i] *= d[i]; }
+          }
+        };
+        if (!BWD) {
 #pragma unroll
           for (int k = 0; k < UPL; ++k) {
-            V::widen(gr[j][k][0], g[k]);
-            V::widen(gr[j][k][1], g[k] + W);
-            turn<W>(HALF, unit[k].pairs, co[k], si[k], g[k], g[k] + W);
-            if (NORM) {
+            if (WEIGHTS == kPerHead) {
+              float pu[W], pv[W];
+              load_weight<T, W, HALF>(P, R, unit[k], min(h + j, h1 - 1), pu, pv);
 #pragma unroll
-              for (int i = 0; i < 2 * W; ++i) {
-                const float xh = x[k][i] * rstd;
-                if (ok) acc[k][i] += g[k][i] * xh;
-                g[k][i] *= w[k][i];
-                dot += g[k][i] * xh;
-                x[k][i] = xh;
-              }
+              for (int i = 0; i < W; ++i) { u[k][i] *= pu[i]; v[k][i] *= pv[i]; }
             }
-          }
-          if (NORM) {
-            for (int o = lanes >> 1; o > 0; o >>= 1) dot += __shfl_xor_sync(kFullMask, dot, o);
-            c = dot * inv_d;
-#pragma unroll
-            for (int k = 0; k < UPL; ++k)
-#pragma unroll
-              for (int i = 0; i < 2 * W; ++i) g[k][i] = rstd * (g[k][i] - x[k][i] * c);
+            turn(k, u[k], v[k]);
           }
         } else {
 #pragma unroll
-          for (int k = 0; k < UPL; ++k) {
-            if (NORM) {
+          for (int k = 0; k < UPL; ++k) turn(k, gu[k], gv[k]);
+          if (NORM) {
+            float dot = 0.f, dou = 0.f;
 #pragma unroll
-              for (int i = 0; i < 2 * W; ++i) x[k][i] = x[k][i] * rstd * w[k][i];
+            for (int k = 0; k < UPL; ++k) {
+              const float* w = held[lane + k * lanes];
+#pragma unroll
+              for (int i = 0; i < W; ++i) {
+                if (ok) {
+                  acc_u[k][i] += gu[k][i] * u[k][i];
+                  acc_v[k][i] += gv[k][i] * v[k][i];
+                }
+                gu[k][i] *= w[i];
+                gv[k][i] *= w[W + i];
+                dot += gu[k][i] * u[k][i];
+                dou += gv[k][i] * v[k][i];
+              }
             }
-            turn<W>(HALF, unit[k].pairs, co[k], si[k], x[k], x[k] + W);
+            const float c = row_sum(dot + dou, lanes) * inv_d;
+#pragma unroll
+            for (int k = 0; k < UPL; ++k)
+#pragma unroll
+              for (int i = 0; i < W; ++i) {        // rstd (g w - xhat c)
+                gu[k][i] = rstd * (gu[k][i] - u[k][i] * c);
+                gv[k][i] = rstd * (gv[k][i] - v[k][i] * c);
+              }
           }
         }
         if (ok) {
 #pragma unroll
-          for (int k = 0; k < UPL; ++k) {
-            const float* y = BWD ? g[k] : x[k];
-            if (unit[k].a >= 0) V::store(op + (h + j) * R.o_sh + unit[k].a, y);
-            if (unit[k].b >= 0) V::store(op + (h + j) * R.o_sh + unit[k].b, y + W);
-          }
+          for (int k = 0; k < UPL; ++k) store<T, W, HALF, FULL>(unit[k], op, BWD ? gu[k] : u[k], BWD ? gv[k] : v[k]);
+          op += R.o_sh;
         }
       }
     }
@@ -247,14 +366,25 @@ __global__ void __launch_bounds__(heads::kThreads, 2) heads_kernel(const HeadsPa
 #pragma unroll
     for (int k = 0; k < UPL; ++k)
 #pragma unroll
-      for (int i = 0; i < 2 * W; ++i) {
-        float s = acc[k][i];
-        for (int o = 16; o >= lanes; o >>= 1) s += __shfl_xor_sync(kFullMask, s, o);
-        const int e = i < W ? unit[k].a : unit[k].b;
-        if ((threadIdx.x & 31) < lanes && e >= 0) fold[wib][e + (i < W ? i : i - W)] = s;
+      for (int i = 0; i < W; ++i) {
+        float su = acc_u[k][i], sv = acc_v[k][i];
+        for (int o = 16; o >= lanes; o >>= 1) {
+          su += __shfl_xor_sync(kFullMask, su, o);
+          sv += __shfl_xor_sync(kFullMask, sv, o);
+        }
+        int eu = unit[k].a + i, ev = unit[k].b + i;
+        if (!HALF && W > 1) {
+          eu = i < FIRST ? unit[k].a + 2 * i : unit[k].b + 2 * (i - FIRST);
+          ev = eu + 1;
+        }
+        const bool has_u = (HALF || i < FIRST ? unit[k].a : unit[k].b) >= 0, has_v = (!HALF && W > 1 ? has_u : unit[k].b >= 0);
+        if ((threadIdx.x & 31) < lanes) {
+          if (has_u) fold[wib][eu] = su;
+          if (has_v) fold[wib][ev] = sv;
+        }
       }
     __syncthreads();
-    float* partial = P.partial + ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * P.d;
+    float* partial = P.partial + (int64_t)blockIdx.x * P.d;
     for (int e = threadIdx.x; e < P.d; e += kThreads) {
       float s = 0.f;
 #pragma unroll
@@ -264,39 +394,41 @@ __global__ void __launch_bounds__(heads::kThreads, 2) heads_kernel(const HeadsPa
   }
 }
 
-// dw of a weight row: the sum of its slots' partials over the blocks, in a fixed order.  blockIdx.y: the weight row (queries'
-// rows first); 32 elements a block, eight threads an element.
+// dw of a weight row: the sum of its slots' partials over their blocks, in a fixed order.  blockIdx.y: the weight row (queries'
+// rows first); 32 elements a block, 32 threads an element.
 template <typename T>
-__global__ void __launch_bounds__(256) heads_dweight_kernel(const HeadsParams P, int blocks) {
-  __shared__ float fold[8][33];
+__global__ void __launch_bounds__(1024) heads_dweight_kernel(const HeadsParams P) {
+  __shared__ float fold[32][33];
+  ptx::grid_wait();
   const int rows_q = P.weight_per_head ? P.part[0].heads : (P.part[0].heads > 0 ? 1 : 0);
   const bool keys = (int)blockIdx.y >= rows_q;
-  const int row = (int)blockIdx.y - (keys ? rows_q : 0);
-  const int first = (keys ? P.slots[0] : 0) + (P.weight_per_head ? row : 0);      // per head: one head a slot
-  const int64_t count = (int64_t)(P.weight_per_head ? 1 : P.slots[keys]) * blocks;
+  const int row = (int)blockIdx.y - (keys ? rows_q : 0), blocks = P.blocks[keys];
+  const int64_t first = (keys ? (int64_t)P.slots[0] * P.blocks[0] : 0) + (P.weight_per_head ? (int64_t)row * blocks : 0);
+  const int count = (P.weight_per_head ? 1 : P.slots[keys]) * blocks;
   const int e = blockIdx.x * 32 + (threadIdx.x & 31), part = threadIdx.x >> 5;
   float s = 0.f;
   if (e < P.d) {
-    const float* src = P.partial + (int64_t)first * blocks * P.d + e;
-#pragma unroll 8
-    for (int64_t r = part; r < count; r += 8) s += src[r * P.d];
+    const float* src = P.partial + first * P.d + e;
+#pragma unroll 4
+    for (int r = part; r < count; r += 32) s += src[(int64_t)r * P.d];
   }
   fold[part][threadIdx.x & 31] = s;
   __syncthreads();
-  if (part == 0 && e < P.d) {
-#pragma unroll
-    for (int k = 1; k < 8; ++k) s += fold[k][threadIdx.x & 31];
+  // a warp adds up the 32 threads of one element
+  s = warp_sum(fold[threadIdx.x & 31][part]);
+  const int out = blockIdx.x * 32 + part;
+  if ((threadIdx.x & 31) == 0 && out < P.d) {
     void* dw = P.part[keys].dweight;
-    const int64_t at = (int64_t)row * P.d + e;
+    const int64_t at = (int64_t)row * P.d + out;
     if (P.weight_f32) ((float*)dw)[at] = s;
     else ((T*)dw)[at] = Elem<T>::from_float(s);
   }
 }
 
-// Widest vector that every row's start, the row length and the layout's second half allow
+// Widest vector that every row's start, the row length and the rotated part allow
 static int vector_width(const HeadsParams& P, int size, bool backward) {
   uint64_t all = (uint64_t)16 | (uint64_t)P.d * size;
-  if (P.half) all |= (uint64_t)P.rotary_dim / 2 * size;
+  all |= (uint64_t)(P.half ? P.rotary_dim / 2 : P.rotary_dim) * size;
   for (const HeadRows& r : P.part) {
     if (r.heads == 0) continue;
     all |= reinterpret_cast<uintptr_t>(r.out) | (uint64_t)(r.o_sb | r.o_sh | r.o_sn) * size;
@@ -307,19 +439,27 @@ static int vector_width(const HeadsParams& P, int size, bool backward) {
   return (int)(bytes / size);
 }
 
-// Blocks over the tokens and heads a slot
-static void heads_grid(const HeadsParams& P, bool backward, int groups, int* per_slot, int64_t* blocks) {
+// Heads a slot, and blocks over the tokens for the slots of the queries and of the keys.  `one`: a head a slot.
+static int heads_grid(HeadsParams& P, bool persistent, bool one, int groups) {
   const int64_t all = ((int64_t)P.batch * P.seq + groups - 1) / groups;
-  int per = P.norm && P.weight_per_head ? 1 : 8;
+  int per = one ? 1 : HEADS_PER;
   auto slots = [&](int p) { return (int64_t)(P.part[0].heads + p - 1) / p + (P.part[1].heads + p - 1) / p; };
-  // few tokens: heads go to blocks of their own until every SM has two
-  while (per > 1 && all * slots(per) < 2 * 148) per /= 2;
-  *per_slot = per;
-  *blocks = all;
-  if (P.norm && backward) {           // as many blocks as are resident, each with a partial weight gradient
-    const int64_t most = (2 * 148 + slots(per) - 1) / slots(per);
-    if (*blocks > most) *blocks = most;
+  // one set of angles serves a slot's heads; few tokens: heads go to blocks of their own until every SM has several
+  while (per > 1 && all * slots(per) < (persistent ? HEADS_R : HEADS_W) * 148) per /= 2;
+  int64_t total = 0;
+  for (int i = 0; i < 2; ++i) {
+    P.slots[i] = (P.part[i].heads + per - 1) / per;
+    // with partial weight gradients as many blocks as are resident at once, by the parts' share of the heads
+    const int64_t share = (int64_t)HEADS_R * 148 * P.part[i].heads / (P.part[0].heads + P.part[1].heads);
+    const int64_t most = P.slots[i] > 0 ? (share + P.slots[i] - 1) / P.slots[i] : 1;
+    const int64_t blocks = persistent && all > most ? (most > 0 ? most : 1) : all;
+    if (blocks > 0x7fffffffLL) return fail(NSA_ERR_SHAPE, "heads: too many tokens for one launch");
+    P.blocks[i] = (int)blocks;
+    total += blocks * P.slots[i];
   }
+  P.per_slot = per;
+  if (total > 0x7fffffffLL) return fail(NSA_ERR_SHAPE, "heads: too many heads and tokens for one launch");
+  return NSA_OK;
 }
 
 static int lane_shift(const HeadsParams& P, int W, int* units_per_lane) {
@@ -332,42 +472,61 @@ static int lane_shift(const HeadsParams& P, int W, int* units_per_lane) {
 
 int64_t heads_partial_floats(const HeadsParams& P0) {
   if (!P0.norm) return 0;
-  // the most that any vector width asks for: 256 groups a block give the fewest blocks, 8 the most
-  const int64_t slots = P0.part[0].heads + P0.part[1].heads;
-  return (2 * 148 + slots) * P0.d;
+  // blocks: the share of each part, rounded up once for each slot
+  return (HEADS_R * 148 + 2 * ((int64_t)P0.part[0].heads + P0.part[1].heads)) * P0.d;
 }
 
-template <typename T, int W, int UPL, bool NORM, bool BWD>
+template <typename T, int W, int UPL, int WEIGHTS, bool BWD>
 static int launch_heads_w(HeadsParams& P, cudaStream_t stream) {
-  int units = 0, per = 0;
-  int64_t blocks = 0;
+  using heads::kNone;
+  int units = 0;
   P.lane_shift = lane_shift(P, W, &units);
   if (units > UPL) return fail(NSA_ERR_UNSUPPORTED, "heads: dim_head is too large for rows that lie on such boundaries");
-  heads_grid(P, BWD, heads::kThreads >> P.lane_shift, &per, &blocks);
-  P.per_slot = per;
-  for (int i = 0; i < 2; ++i) P.slots[i] = (P.part[i].heads + per - 1) / per;
-  const int slots = P.slots[0] + P.slots[1];
-  if (blocks > 0x7fffffffLL || slots > 65535) return fail(NSA_ERR_SHAPE, "heads: too many heads or tokens for one launch");
-  const dim3 grid((unsigned)blocks, (unsigned)slots);
-  if (P.half) heads_kernel<T, W, UPL, true, NORM, BWD><<<grid, heads::kThreads, 0, stream>>>(P);
-  else heads_kernel<T, W, UPL, false, NORM, BWD><<<grid, heads::kThreads, 0, stream>>>(P);
-  count_launches(1);
-  if (NORM && BWD) {
+  constexpr bool partials = WEIGHTS != kNone && BWD;
+  const int rc = heads_grid(P, partials, partials && WEIGHTS == heads::kPerHead, heads::kThreads >> P.lane_shift);
+  if (rc != NSA_OK) return rc;
+  const unsigned grid = (unsigned)(P.slots[0] * P.blocks[0] + P.slots[1] * P.blocks[1]);
+  const bool full = W * (int)sizeof(T) == 16 && P.d == (2 * W << P.lane_shift);      // the usual heads, in the widest vectors
+  constexpr bool wide = W * sizeof(T) == 16;
+  if (full && P.half) heads_kernel<T, W, UPL, true, WEIGHTS, BWD, wide><<<grid, heads::kThreads, 0, stream>>>(P);
+  else if (full) heads_kernel<T, W, UPL, false, WEIGHTS, BWD, wide><<<grid, heads::kThreads, 0, stream>>>(P);
+  else if (P.half) heads_kernel<T, W, UPL, true, WEIGHTS, BWD, false><<<grid, heads::kThreads, 0, stream>>>(P);
+  else heads_kernel<T, W, UPL, false, WEIGHTS, BWD, false><<<grid, heads::kThreads, 0, stream>>>(P);
+  cudaError_t err = cudaGetLastError();
+  if (partials && err == cudaSuccess) {
     const int rows = P.weight_per_head ? P.part[0].heads + P.part[1].heads : (P.part[0].heads > 0) + (P.part[1].heads > 0);
-    heads_dweight_kernel<T><<<dim3((unsigned)(P.d + 31) / 32, (unsigned)rows), 256, 0, stream>>>(P, (int)blocks);
-    count_launches(1);
+    if (rows > 65535) return fail(NSA_ERR_SHAPE, "heads: more than 65535 weight rows");
+    cudaLaunchConfig_t config = {};      // starts while the last blocks of the kernel before it are at work
+    config.gridDim = dim3((unsigned)(P.d + 31) / 32, (unsigned)rows);
+    config.blockDim = dim3(1024);
+    config.stream = stream;
+    cudaLaunchAttribute overlap = {};
+    overlap.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    overlap.val.programmaticStreamSerializationAllowed = 1;
+    config.attrs = &overlap;
+    config.numAttrs = 1;
+    err = cudaLaunchKernelEx(&config, heads_dweight_kernel<T>, P);
   }
-  const cudaError_t err = cudaGetLastError();
-  return err == cudaSuccess ? NSA_OK : fail((int)err, cudaGetErrorString(err));
+  if (err != cudaSuccess) return fail((int)err, cudaGetErrorString(err));
+  count_launches(partials ? 2 : 1);
+  return NSA_OK;
 }
 
-template <typename T, bool NORM, bool BWD>
+template <typename T, int WEIGHTS, bool BWD>
 static int launch_heads_typed(HeadsParams& P, cudaStream_t stream) {
   constexpr int kMost = 16 / (int)sizeof(T);
   const int W = vector_width(P, sizeof(T), BWD);
-  if (W >= kMost) return launch_heads_w<T, kMost, 1, NORM, BWD>(P, stream);
-  if (W >= kMost / 2) return launch_heads_w<T, kMost / 2, kMost / 2 >= 4 ? 1 : 2, NORM, BWD>(P, stream);
-  return launch_heads_w<T, 1, 4, NORM, BWD>(P, stream);
+  if (W >= kMost) return launch_heads_w<T, kMost, 1, WEIGHTS, BWD>(P, stream);
+  if (W >= kMost / 2) return launch_heads_w<T, kMost / 2, kMost / 2 >= 4 ? 1 : 2, WEIGHTS, BWD>(P, stream);
+  return launch_heads_w<T, 1, 4, WEIGHTS, BWD>(P, stream);
+}
+
+template <typename T>
+static int launch_heads_dir(HeadsParams& P, bool backward, cudaStream_t stream) {
+  using namespace heads;
+  if (!P.norm) return backward ? launch_heads_typed<T, kNone, true>(P, stream) : launch_heads_typed<T, kNone, false>(P, stream);
+  if (!P.weight_per_head) return backward ? launch_heads_typed<T, kShared, true>(P, stream) : launch_heads_typed<T, kShared, false>(P, stream);
+  return backward ? launch_heads_typed<T, kPerHead, true>(P, stream) : launch_heads_typed<T, kPerHead, false>(P, stream);
 }
 
 int launch_heads(HeadsParams& P, int dtype, bool backward, cudaStream_t stream) {
@@ -381,12 +540,7 @@ int launch_heads(HeadsParams& P, int dtype, bool backward, cudaStream_t stream) 
     }
     return NSA_OK;
   }
-  if (dtype == NSA_F32) {
-    if (P.norm) return backward ? launch_heads_typed<float, true, true>(P, stream) : launch_heads_typed<float, true, false>(P, stream);
-    return backward ? launch_heads_typed<float, false, true>(P, stream) : launch_heads_typed<float, false, false>(P, stream);
-  }
-  if (P.norm) return backward ? launch_heads_typed<__nv_bfloat16, true, true>(P, stream) : launch_heads_typed<__nv_bfloat16, true, false>(P, stream);
-  return backward ? launch_heads_typed<__nv_bfloat16, false, true>(P, stream) : launch_heads_typed<__nv_bfloat16, false, false>(P, stream);
+  return dtype == NSA_F32 ? launch_heads_dir<float>(P, backward, stream) : launch_heads_dir<__nv_bfloat16>(P, backward, stream);
 }
 
 }  // namespace nsa

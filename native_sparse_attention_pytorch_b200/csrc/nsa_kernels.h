@@ -126,7 +126,7 @@ struct HeadsParams {
   float* partial;        // backward with norm: heads_partial_floats
   int batch, seq, d, rotary_dim, half, norm, weight_f32, weight_per_head, pos_i64;
   float magnitude, eps;
-  int lane_shift, per_slot, slots[2];   // filled in by launch_heads
+  int lane_shift, per_slot, slots[2], blocks[2];   // filled in by launch_heads
 };
 int64_t heads_partial_floats(const HeadsParams& P);
 int launch_heads(HeadsParams& P, int dtype, bool backward, cudaStream_t stream);
