@@ -11,7 +11,7 @@
 // Work.  A row (one head of one token) belongs to 2^k neighbouring lanes, a lane to `units` of two vectors of W elements, whose
 // elements are W pairs (u, v): with the half layout u from one vector and v from the other, else even and odd elements of both.
 // A group of lanes goes through up to `per_slot` heads of a token (a slot: heads of the queries or of the keys), kBatch of them in
-// flight.  What bounds it is the traffic: x (and dy) in, y (or dx) out.
+// flight, two values an instruction.  What bounds it is the traffic: x (and dy) in, y (or dx) out.
 
 #include "nsa_common.cuh"
 #include "nsa_kernels.h"
@@ -26,6 +26,8 @@ namespace nsa {
 #define HEADS_PER 32
 #define HEADS_W 6
 #define HEADS_R 4
+#define HEADS_ST 4
+#define HEADS_MR 4
 #endif
 namespace heads {
 
@@ -140,15 +142,55 @@ __device__ __forceinline__ void store(const Unit& t, T* row, const float* u, con
   if (FULL || t.b >= 0) Vec<T, W>::store(row + t.b, y);
 }
 
-// (u, v) -> (u cu - v cv, v dv + u du): N pairs
+// Products and sums over W values, two an instruction (each rounded as a single one)
+template <int W>
+__device__ __forceinline__ void mul(const float* a, const float* b, float* r) {
+  if constexpr (W == 1) r[0] = a[0] * b[0];
+  else
+#pragma unroll
+    for (int i = 0; i < W; i += 2) ptx::unpack2(ptx::mul2(ptx::pack2(a[i], a[i + 1]), ptx::pack2(b[i], b[i + 1])), r[i], r[i + 1]);
+}
+template <int W>
+__device__ __forceinline__ void fma(const float* a, const float* b, const float* c, float* r) {
+  if constexpr (W == 1) r[0] = a[0] * b[0] + c[0];
+  else
+#pragma unroll
+    for (int i = 0; i < W; i += 2)
+      ptx::unpack2(ptx::fma2(ptx::pack2(a[i], a[i + 1]), ptx::pack2(b[i], b[i + 1]), ptx::pack2(c[i], c[i + 1])), r[i], r[i + 1]);
+}
+template <int W>
+__device__ __forceinline__ void scale(float b, float* r) {
+  if constexpr (W == 1) r[0] *= b;
+  else
+#pragma unroll
+    for (int i = 0; i < W; i += 2) ptx::unpack2(ptx::mul2(ptx::pack2(r[i], r[i + 1]), ptx::pack2(b, b)), r[i], r[i + 1]);
+}
+// r += a b
+template <int W>
+__device__ __forceinline__ void add_scaled(const float* a, float b, float* r) {
+  if constexpr (W == 1) r[0] += a[0] * b;
+  else
+#pragma unroll
+    for (int i = 0; i < W; i += 2) ptx::unpack2(ptx::fma2(ptx::pack2(a[i], a[i + 1]), ptx::pack2(b, b), ptx::pack2(r[i], r[i + 1])), r[i], r[i + 1]);
+}
+// sum += a b, even and odd places apart
+template <int W>
+__device__ __forceinline__ void add_dot(const float* a, const float* b, float (&sum)[2]) {
+  if constexpr (W == 1) sum[0] += a[0] * b[0];
+  else
+#pragma unroll
+    for (int i = 0; i < W; i += 2)
+      ptx::unpack2(ptx::fma2(ptx::pack2(a[i], a[i + 1]), ptx::pack2(b[i], b[i + 1]), ptx::pack2(sum[0], sum[1])), sum[0], sum[1]);
+}
+
+// (u, v) -> (u cu + v cv, v dv + u du): N pairs
 template <int N>
 __device__ __forceinline__ void rotate(float* u, float* v, const float* cu, const float* cv, const float* dv, const float* du) {
-#pragma unroll
-  for (int i = 0; i < N; ++i) {
-    const float a = u[i] * cu[i] - v[i] * cv[i];
-    v[i] = v[i] * dv[i] + u[i] * du[i];
-    u[i] = a;
-  }
+  float a[N], b[N];
+  mul<N>(v, cv, a);
+  mul<N>(u, du, b);
+  fma<N>(u, cu, a, u);
+  fma<N>(v, dv, b, v);
 }
 
 // Sine and cosine of a phase, 2^64 to the turn.  The nearest quarter turn is taken off in integers; what is left, at most pi / 4, goes
@@ -178,7 +220,7 @@ __device__ __forceinline__ float row_sum(float v, int lanes) {
 // WEIGHTS: kNone (no norm), kShared, kPerHead
 // FULL: every lane has both vectors of every unit
 template <typename T, int W, int UPL, bool HALF, int WEIGHTS, bool BWD, bool FULL>
-__global__ void __launch_bounds__(heads::kThreads, HEADS_MB) heads_kernel(const HeadsParams P) {
+__global__ void __launch_bounds__(heads::kThreads, FULL && WEIGHTS != heads::kNone ? HEADS_MR : HEADS_MB) heads_kernel(const HeadsParams P) {
   using namespace heads;
   using V = Vec<T, W>;
   typedef typename V::Raw Raw;
@@ -186,10 +228,15 @@ __global__ void __launch_bounds__(heads::kThreads, HEADS_MB) heads_kernel(const 
   constexpr bool XIN = !BWD || NORM;                              // x is read
   constexpr bool FOLD = WEIGHTS == kShared && !BWD;               // the weights are part of the rotation's factors
   constexpr bool ONE = WEIGHTS == kPerHead && BWD;                // one head a slot, whose weight gradient stays in registers
-  constexpr int kBatch = UPL > 1 || ONE ? 1 : (BWD && NORM ? HEADS_HN : HEADS_HB);     // heads in flight
+  constexpr bool RING = FULL && NORM;                             // rows come through shared memory
+  constexpr int kVecs = BWD ? 4 : 2, kStages = RING ? HEADS_ST : 1;
+  constexpr int kBatch = UPL > 1 || ONE || RING ? 1 : (BWD && NORM ? HEADS_HN : HEADS_HB);     // heads in flight
   constexpr int FIRST = first_pairs<W, HALF>();
   __shared__ float fold[NORM && BWD ? kThreads / 32 : 1][NORM && BWD ? kHeadsMaxDim : 1];
   __shared__ __align__(16) float held[NORM && BWD ? 32 * UPL : 1][NORM && BWD ? 2 * W : 1];   // the backward's weights, unit by unit
+
+  // every thread's own places: 16 bytes of each vector of kStages rows
+  __shared__ __align__(16) uint4 places[RING ? kStages * kVecs * kThreads : 1];
 
   ptx::grid_allow_next();
   const int lanes = 1 << P.lane_shift, lane = threadIdx.x & (lanes - 1);
@@ -217,14 +264,63 @@ __global__ void __launch_bounds__(heads::kThreads, HEADS_MB) heads_kernel(const 
 
   const unsigned tokens = (unsigned)P.batch * (unsigned)P.seq;
   const float inv_d = 1.f / (float)P.d;
+  const unsigned step = blocks * groups;
+  auto position = [&](unsigned token) {
+    const unsigned b = token / (unsigned)P.seq, n = token - b * (unsigned)P.seq;
+    if (P.positions == nullptr) return P.offset + n;
+    const int64_t at = (int64_t)b * P.pos_sb + n;
+    return P.offset + (P.pos_i64 ? ((const int64_t*)P.positions)[at] : (int64_t)((const int32_t*)P.positions)[at]);
+  };
+  auto row_at = [&](const void* base, int64_t sb, int64_t sh, int64_t sn, unsigned token) {     // the slot's first head
+    const unsigned b = token / (unsigned)P.seq, n = token - b * (unsigned)P.seq;
+    return (T*)base + (int64_t)b * sb + (int64_t)n * sn + (int64_t)h0 * sh;
+  };
+
+  // RING: rows are on their way kStages - 1 heads ahead, past the end of a token into the next one
+  const uint32_t place = ptx::smem_u32(places + threadIdx.x);
+  unsigned far_token = at_block * groups + group;
+  int far_head = h0, far_stage = 0, stage = 0;
+  const T *far_x = nullptr, *far_g = nullptr;
+  auto far_locate = [&]() {
+    if (far_token >= tokens) return;
+    far_x = row_at(R.x, R.x_sb, R.x_sh, R.x_sn, far_token);
+    if (BWD) far_g = row_at(R.dy, R.dy_sb, R.dy_sh, R.dy_sn, far_token);
+  };
+  auto far_fetch = [&]() {
+    if (far_token < tokens) {
+      const uint32_t at = place + far_stage * (kVecs * kThreads * 16);
+      ptx::cp_async16(at, far_x + unit[0].a, 16);
+      ptx::cp_async16(at + kThreads * 16, far_x + unit[0].b, 16);
+      if (BWD) {
+        ptx::cp_async16(at + 2 * kThreads * 16, far_g + unit[0].a, 16);
+        ptx::cp_async16(at + 3 * kThreads * 16, far_g + unit[0].b, 16);
+      }
+    }
+    ptx::cp_async_commit();
+    far_stage = far_stage + 1 == kStages ? 0 : far_stage + 1;
+    if (++far_head < h1) {
+      far_x += R.x_sh;
+      if (BWD) far_g += R.dy_sh;
+    } else {
+      far_head = h0;
+      far_token += step;
+      far_locate();
+    }
+  };
+  if (RING) {
+    far_locate();
+#pragma unroll 1
+    for (int i = 0; i < kStages - 1; ++i) far_fetch();
+  }
+  int64_t next_pos = position(min(at_block * groups + group, tokens - 1));
+
   // every lane of a warp takes part in the sums over a row: groups without a token go along with nothing to load
-  for (unsigned first = at_block * groups; first < tokens; first += blocks * groups) {
+  for (unsigned first = at_block * groups; first < tokens; first += step) {
     const unsigned token = first + group;
     const bool live = token < tokens;
-    const unsigned b = live ? token / (unsigned)P.seq : 0, n = live ? token - b * (unsigned)P.seq : 0;
-    const T* xp = XIN ? (const T*)R.x + (int64_t)b * R.x_sb + (int64_t)n * R.x_sn + (int64_t)h0 * R.x_sh : nullptr;
-    const T* gp = BWD ? (const T*)R.dy + (int64_t)b * R.dy_sb + (int64_t)n * R.dy_sn + (int64_t)h0 * R.dy_sh : nullptr;
-    T* op = (T*)R.out + (int64_t)b * R.o_sb + (int64_t)n * R.o_sn + (int64_t)h0 * R.o_sh;
+    const T* xp = XIN && !RING ? row_at(R.x, R.x_sb, R.x_sh, R.x_sn, live ? token : 0) : nullptr;
+    const T* gp = BWD && !RING ? row_at(R.dy, R.dy_sb, R.dy_sh, R.dy_sn, live ? token : 0) : nullptr;
+    T* op = row_at(R.out, R.o_sb, R.o_sh, R.o_sn, live ? token : 0);
     Raw xr[kBatch][UPL][2], gr[BWD ? kBatch : 1][UPL][2];
     // the next head's values into place j; beyond the slot's heads (and, with FULL, for groups without a token) those of the last
     // one, of which nothing is kept
@@ -247,15 +343,13 @@ __global__ void __launch_bounds__(heads::kThreads, HEADS_MB) heads_kernel(const 
         if (BWD) gp += R.dy_sh;
       }
     };
+    if (!RING)
 #pragma unroll
-    for (int j = 0; j < kBatch; ++j) fetch(j);                 // under way while the angles are formed
-    int64_t pos = P.offset + n;
-    if (P.positions != nullptr) {
-      const int64_t at = (int64_t)b * P.pos_sb + n;
-      pos = P.offset + (P.pos_i64 ? ((const int64_t*)P.positions)[at] : (int64_t)((const int32_t*)P.positions)[at]);
-    }
-    // factors of the rotation: u' = u cu - v cv, v' = v dv + u du; with the weights in them (FOLD), else two sets are enough
-    float cu[UPL][W], cv[UPL][W], dv[FOLD ? UPL : 1][W], du[FOLD ? UPL : 1][W];
+      for (int j = 0; j < kBatch; ++j) fetch(j);               // under way while the angles are formed
+    const int64_t pos = next_pos;
+    if (first + step < tokens) next_pos = position(min(token + step, tokens - 1));
+    // factors of the rotation: u' = u cu + v cv, v' = v dv + u du, with the weights in them (FOLD; else dv = cu)
+    float cu[UPL][W], cv[UPL][W], dv[FOLD ? UPL : 1][W], du[UPL][W];
 #pragma unroll
     for (int k = 0; k < UPL; ++k)
 #pragma unroll
@@ -266,11 +360,11 @@ __global__ void __launch_bounds__(heads::kThreads, HEADS_MB) heads_kernel(const 
           co *= P.magnitude;
           si *= BWD ? -P.magnitude : P.magnitude;
         }
-        cu[k][i] = co; cv[k][i] = si;
+        cu[k][i] = co; cv[k][i] = -si; du[k][i] = si;
         if (FOLD) {
           const int f = FOLD ? k : 0;
-          dv[f][i] = wv[f][i] * co; du[f][i] = wu[f][i] * si;
-          cu[k][i] *= wu[f][i]; cv[k][i] *= wv[f][i];
+          dv[f][i] = wv[f][i] * co;
+          cu[k][i] *= wu[f][i]; cv[k][i] *= wv[f][i]; du[k][i] *= wu[f][i];
         }
       }
     for (int h = h0; h < h1; h += kBatch) {
@@ -280,30 +374,41 @@ __global__ void __launch_bounds__(heads::kThreads, HEADS_MB) heads_kernel(const 
         float u[UPL][W], v[UPL][W], gu[BWD ? UPL : 1][W], gv[BWD ? UPL : 1][W];          // x, dy; then what is stored
 #pragma unroll
         for (int k = 0; k < UPL; ++k) {
-          if (XIN) split<T, W, HALF>(xr[j][k][0], xr[j][k][1], u[k], v[k]);
-          if (BWD) split<T, W, HALF>(gr[j][k][0], gr[j][k][1], gu[k], gv[k]);
+          if constexpr (RING) {
+            ptx::cp_async_wait<kStages - 2>();
+            const uint32_t at = place + stage * (kVecs * kThreads * 16);
+            uint4 raw[kVecs];
+#pragma unroll
+            for (int i = 0; i < kVecs; ++i) raw[i] = ptx::lds_v4(at + i * (kThreads * 16));
+            split<T, W, HALF>(reinterpret_cast<const Raw&>(raw[0]), reinterpret_cast<const Raw&>(raw[1]), u[k], v[k]);
+            if (BWD) split<T, W, HALF>(reinterpret_cast<const Raw&>(raw[kVecs - 2]), reinterpret_cast<const Raw&>(raw[kVecs - 1]), gu[k], gv[k]);
+            stage = stage + 1 == kStages ? 0 : stage + 1;
+          } else {
+            if (XIN) split<T, W, HALF>(xr[j][k][0], xr[j][k][1], u[k], v[k]);
+            if (BWD) split<T, W, HALF>(gr[j][k][0], gr[j][k][1], gu[k], gv[k]);
+          }
         }
-        if (!ONE) fetch(j);                  // the place is free: the next head's values are on their way meanwhile
+        // the place is free: the next head's values are on their way meanwhile
+        if (RING) far_fetch();
+        else if (!ONE) fetch(j);
         float rstd = 1.f;
         if (NORM) {
-          float ss = 0.f, st = 0.f;
+          float ss[2] = {0.f, 0.f};
 #pragma unroll
-          for (int k = 0; k < UPL; ++k)
-#pragma unroll
-            for (int i = 0; i < W; ++i) { ss += u[k][i] * u[k][i]; st += v[k][i] * v[k][i]; }
-          rstd = rsqrtf(row_sum(ss + st, lanes) * inv_d + P.eps);
-#pragma unroll
-          for (int k = 0; k < UPL; ++k)
-#pragma unroll
-            for (int i = 0; i < W; ++i) { u[k][i] *= rstd; v[k][i] *= rstd; }
+          for (int k = 0; k < UPL; ++k) {
+            add_dot<W>(u[k], u[k], ss);
+            add_dot<W>(v[k], v[k], ss);
+          }
+          rstd = rsqrtf(row_sum(ss[0] + ss[1], lanes) * inv_d + P.eps);
         }
         auto turn = [&](int k, float* p, float* q) {
           const float* d = FOLD ? dv[FOLD ? k : 0] : cu[k];
-          const float* e = FOLD ? du[FOLD ? k : 0] : cv[k];
-          if (unit[k].rot_a && unit[k].rot_b) rotate<W>(p, q, cu[k], cv[k], d, e);
+          if (unit[k].rot_a && unit[k].rot_b) rotate<W>(p, q, cu[k], cv[k], d, du[k]);
           else {                             // a pair that is not rotated must not be multiplied with the other's zero
-            if (unit[k].rot_a) rotate<FIRST>(p, q, cu[k], cv[k], d, e);
-            if (unit[k].rot_b && FIRST < W) rotate<W - FIRST>(p + FIRST, q + FIRST, cu[k] + FIRST, cv[k] + FIRST, d + FIRST, e + FIRST);
+            if (unit[k].rot_a) rotate<FIRST>(p, q, cu[k], cv[k], d, du[k]);
+            if constexpr (FIRST < W) {
+              if (unit[k].rot_b) rotate<W - FIRST>(p + FIRST, q + FIRST, cu[k] + FIRST, cv[k] + FIRST, d + FIRST, du[k] + FIRST);
+            }
             if (FOLD)
 #pragma unroll
               for (int i = 0; i < W; ++i)
@@ -313,11 +418,15 @@ __global__ void __launch_bounds__(heads::kThreads, HEADS_MB) heads_kernel(const 
         if (!BWD) {
 #pragma unroll
           for (int k = 0; k < UPL; ++k) {
+            if (NORM) {
+              scale<W>(rstd, u[k]);
+              scale<W>(rstd, v[k]);
+            }
             if (WEIGHTS == kPerHead) {
               float pu[W], pv[W];
               load_weight<T, W, HALF>(P, R, unit[k], min(h + j, h1 - 1), pu, pv);
-#pragma unroll
-              for (int i = 0; i < W; ++i) { u[k][i] *= pu[i]; v[k][i] *= pv[i]; }
+              mul<W>(u[k], pu, u[k]);
+              mul<W>(v[k], pv, v[k]);
             }
             turn(k, u[k], v[k]);
           }
@@ -325,30 +434,28 @@ __global__ void __launch_bounds__(heads::kThreads, HEADS_MB) heads_kernel(const 
 #pragma unroll
           for (int k = 0; k < UPL; ++k) turn(k, gu[k], gv[k]);
           if (NORM) {
-            float dot = 0.f, dou = 0.f;
+            // g rstd in place of g: dw += g x, dx = g w - x rstd^2 mean(g w x)
+            float dot[2] = {0.f, 0.f};
 #pragma unroll
             for (int k = 0; k < UPL; ++k) {
               const float* w = held[lane + k * lanes];
-#pragma unroll
-              for (int i = 0; i < W; ++i) {
-                if (ok) {
-                  acc_u[k][i] += gu[k][i] * u[k][i];
-                  acc_v[k][i] += gv[k][i] * v[k][i];
-                }
-                gu[k][i] *= w[i];
-                gv[k][i] *= w[W + i];
-                dot += gu[k][i] * u[k][i];
-                dou += gv[k][i] * v[k][i];
+              scale<W>(rstd, gu[k]);
+              scale<W>(rstd, gv[k]);
+              if (ok) {
+                fma<W>(gu[k], u[k], acc_u[k], acc_u[k]);
+                fma<W>(gv[k], v[k], acc_v[k], acc_v[k]);
               }
+              mul<W>(gu[k], w, gu[k]);
+              mul<W>(gv[k], w + W, gv[k]);
+              add_dot<W>(gu[k], u[k], dot);
+              add_dot<W>(gv[k], v[k], dot);
             }
-            const float c = row_sum(dot + dou, lanes) * inv_d;
+            const float c = -rstd * rstd * (row_sum(dot[0] + dot[1], lanes) * inv_d);
 #pragma unroll
-            for (int k = 0; k < UPL; ++k)
-#pragma unroll
-              for (int i = 0; i < W; ++i) {        // rstd (g w - xhat c)
-                gu[k][i] = rstd * (gu[k][i] - u[k][i] * c);
-                gv[k][i] = rstd * (gv[k][i] - v[k][i] * c);
-              }
+            for (int k = 0; k < UPL; ++k) {
+              add_scaled<W>(u[k], c, gu[k]);
+              add_scaled<W>(v[k], c, gv[k]);
+            }
           }
         }
         if (ok) {
