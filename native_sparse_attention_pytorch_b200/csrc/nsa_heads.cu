@@ -25,8 +25,9 @@ namespace nsa {
 #define HEADS_HB 4
 #define HEADS_PER 32
 #define HEADS_W 6
-#define HEADS_R 4
-#define HEADS_ST 4
+#define HEADS_R 8
+#define HEADS_ST 5
+#define HEADS_STB 3
 #define HEADS_MR 4
 #endif
 namespace heads {
@@ -229,7 +230,7 @@ __global__ void __launch_bounds__(heads::kThreads, FULL && WEIGHTS != heads::kNo
   constexpr bool FOLD = WEIGHTS == kShared && !BWD;               // the weights are part of the rotation's factors
   constexpr bool ONE = WEIGHTS == kPerHead && BWD;                // one head a slot, whose weight gradient stays in registers
   constexpr bool RING = FULL && NORM;                             // rows come through shared memory
-  constexpr int kVecs = BWD ? 4 : 2, kStages = RING ? HEADS_ST : 1;
+  constexpr int kVecs = BWD ? 4 : 2, kStages = RING ? (BWD ? HEADS_STB : HEADS_ST) : 1;
   constexpr int kBatch = UPL > 1 || ONE || RING ? 1 : (BWD && NORM ? HEADS_HN : HEADS_HB);     // heads in flight
   constexpr int FIRST = first_pairs<W, HALF>();
   __shared__ float fold[NORM && BWD ? kThreads / 32 : 1][NORM && BWD ? kHeadsMaxDim : 1];
@@ -502,29 +503,30 @@ __global__ void __launch_bounds__(heads::kThreads, FULL && WEIGHTS != heads::kNo
 }
 
 // dw of a weight row: the sum of its slots' partials over their blocks, in a fixed order.  blockIdx.y: the weight row (queries'
-// rows first); 32 elements a block, 32 threads an element.
+// rows first); eight elements a block, 128 threads an element: the thousand partials of a row are nine loads deep (1155 partials of
+// 64 and 64 elements: 7.8 us with 32 elements a block).
 template <typename T>
 __global__ void __launch_bounds__(1024) heads_dweight_kernel(const HeadsParams P) {
-  __shared__ float fold[32][33];
-  ptx::grid_wait();
+  __shared__ float fold[8][129];
   const int rows_q = P.weight_per_head ? P.part[0].heads : (P.part[0].heads > 0 ? 1 : 0);
   const bool keys = (int)blockIdx.y >= rows_q;
   const int row = (int)blockIdx.y - (keys ? rows_q : 0), blocks = P.blocks[keys];
   const int64_t first = (keys ? (int64_t)P.slots[0] * P.blocks[0] : 0) + (P.weight_per_head ? (int64_t)row * blocks : 0);
   const int count = (P.weight_per_head ? 1 : P.slots[keys]) * blocks;
-  const int e = blockIdx.x * 32 + (threadIdx.x & 31), part = threadIdx.x >> 5;
+  const int e = blockIdx.x * 8 + (threadIdx.x & 7), part = threadIdx.x >> 3;
   float s = 0.f;
+  ptx::grid_wait();
   if (e < P.d) {
     const float* src = P.partial + first * P.d + e;
-#pragma unroll 4
-    for (int r = part; r < count; r += 32) s += src[(int64_t)r * P.d];
+#pragma unroll 10
+    for (int r = part; r < count; r += 128) s += src[(int64_t)r * P.d];
   }
-  fold[part][threadIdx.x & 31] = s;
+  fold[threadIdx.x & 7][part] = s;
   __syncthreads();
-  // a warp adds up the 32 threads of one element
-  s = warp_sum(fold[threadIdx.x & 31][part]);
-  const int out = blockIdx.x * 32 + part;
-  if ((threadIdx.x & 31) == 0 && out < P.d) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, out = blockIdx.x * 8 + warp;
+  if (warp >= 8) return;
+  s = warp_sum((fold[warp][lane] + fold[warp][lane + 32]) + (fold[warp][lane + 64] + fold[warp][lane + 96]));
+  if (lane == 0 && out < P.d) {
     void* dw = P.part[keys].dweight;
     const int64_t at = (int64_t)row * P.d + out;
     if (P.weight_f32) ((float*)dw)[at] = s;
@@ -604,7 +606,7 @@ static int launch_heads_w(HeadsParams& P, cudaStream_t stream) {
     const int rows = P.weight_per_head ? P.part[0].heads + P.part[1].heads : (P.part[0].heads > 0) + (P.part[1].heads > 0);
     if (rows > 65535) return fail(NSA_ERR_SHAPE, "heads: more than 65535 weight rows");
     cudaLaunchConfig_t config = {};      // starts while the last blocks of the kernel before it are at work
-    config.gridDim = dim3((unsigned)(P.d + 31) / 32, (unsigned)rows);
+    config.gridDim = dim3((unsigned)(P.d + 7) / 8, (unsigned)rows);
     config.blockDim = dim3(1024);
     config.stream = stream;
     cudaLaunchAttribute overlap = {};

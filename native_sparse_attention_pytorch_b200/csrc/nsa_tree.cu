@@ -39,18 +39,22 @@ __device__ __forceinline__ int cache_blocks(const TreeParams& P, int b) { return
 template <int KB>
 __device__ __forceinline__ int draft_blocks(const TreeParams& P) { return (P.tokens + KB - 1) / KB; }
 
-// Blocks of all units, by a whole warp
+// Blocks of the units of the sequences before `upto`, and of all, by a whole warp
 template <int KB>
-__device__ int64_t total_blocks(const TreeParams& P, int lane, int upto) {
-  int64_t sum = 0;
-  for (int b0 = 0; b0 < upto; b0 += 32) {
-    const int b = b0 + lane;
-    int64_t n = b < upto ? (int64_t)cache_blocks<KB>(P, b) + draft_blocks<KB>(P) : 0;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(kFullMask, n, o);
-    sum += n;
+__device__ void count_blocks(const TreeParams& P, int lane, int upto, int64_t& before, int64_t& total) {
+  int64_t all = 0, some = 0;
+  for (int b = lane; b < P.batch; b += 32) {
+    const int n = cache_blocks<KB>(P, b) + draft_blocks<KB>(P);
+    all += n;
+    some += b < upto ? n : 0;
   }
-  return sum * P.kv_heads;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    all += __shfl_xor_sync(kFullMask, all, o);
+    some += __shfl_xor_sync(kFullMask, some, o);
+  }
+  total = all * P.kv_heads;
+  before = some * P.kv_heads;
 }
 
 // Where a piece of the row of blocks begins: sequence and its first block
@@ -80,7 +84,18 @@ __device__ Place place_of(const TreeParams& P, int lane, int64_t block) {
   return at;
 }
 
-__device__ __forceinline__ int64_t piece_begin(int64_t total, int g, int groups) { return total * g / groups; }
+// The groups that have blocks: no more than there are blocks, so that none of them is without
+__device__ __forceinline__ int busy_groups(const TreeParams& P, int64_t total) { return (int)min((int64_t)P.groups, total); }
+// x / y; a division of 64-bit numbers takes some hundred instructions
+__device__ __forceinline__ int64_t quotient(int64_t x, int y) {
+  return (uint64_t)x >> 32 ? x / y : (int64_t)((uint32_t)x / (uint32_t)y);
+}
+__device__ __forceinline__ int64_t piece_begin(int64_t total, int g, int groups) { return quotient(total * g, groups); }
+// The group that has block x: the last whose piece begins at or before it
+__device__ __forceinline__ int group_of(int64_t total, int64_t x, int groups) {
+  const int64_t y = (x + 1) * groups - 1;
+  return (uint64_t)(y | total) >> 32 ? (int)(y / total) : (int)((uint32_t)y / (uint32_t)total);
+}
 
 __device__ __forceinline__ bool sees(const TreeParams& P, int b, int t, int u) {
   return P.mask != nullptr ? P.mask[b * P.m_sb + t * P.m_st + u] != 0 : u <= t;
@@ -130,9 +145,11 @@ __global__ void __launch_bounds__(tree_simt::kThreads, 2) tree_simt_kernel(const
   const int rows = P.tokens * P.G, row0 = tile * RT;
 
   ptx::grid_allow_next();
-  const int64_t total = total_blocks<kKeys>(P, lane, P.batch);
-  const int64_t begin = piece_begin(total, group, P.groups), end = piece_begin(total, group + 1, P.groups);
-  if (begin >= end) return;
+  int64_t before, total;
+  count_blocks<kKeys>(P, lane, 0, before, total);
+  const int groups = busy_groups(P, total);
+  if (group >= groups) return;
+  const int64_t begin = piece_begin(total, group, groups), end = piece_begin(total, group + 1, groups);
   Place at = place_of<kKeys>(P, lane, begin);
   const float scale2 = P.scale * kLog2e;
 
@@ -167,7 +184,7 @@ __global__ void __launch_bounds__(tree_simt::kThreads, 2) tree_simt_kernel(const
   for (int64_t at_block = begin; at_block < end;) {
     // the unit at_block lies in, and this piece's blocks of it
     const int cached = cache_blocks<kKeys>(P, at.b), per_unit = cached + draft_blocks<kKeys>(P), length = length_of(P, at.b);
-    const int h = (int)((at_block - at.base) / per_unit);
+    const int h = (int)quotient(at_block - at.base, per_unit);
     const int64_t unit0 = at.base + (int64_t)h * per_unit;
     const int j0 = (int)(at_block - unit0), j1 = (int)min((int64_t)per_unit, end - unit0);
 
@@ -360,8 +377,6 @@ struct Walk {
   int64_t base, at, end, unit0;
   // by a whole warp
   __device__ void begin(const TreeParams& P, int lane, int group) {
-    int64_t total = 0;
-    Place p = {0, 0};
     if (P.batch <= 32) {                  // one look at the lengths
       const int64_t n = lane < P.batch ? ((int64_t)cache_blocks<KB>(P, lane) + draft_blocks<KB>(P)) * P.kv_heads : 0;
       int64_t upto = n;
@@ -370,19 +385,23 @@ struct Walk {
         const int64_t v = __shfl_up_sync(kFullMask, upto, o);
         if (lane >= o) upto += v;
       }
-      total = __shfl_sync(kFullMask, upto, 31);
-      at = piece_begin(total, group, P.groups);
+      set_piece(P, __shfl_sync(kFullMask, upto, 31), group);
       const unsigned past = __ballot_sync(kFullMask, upto > at && lane < P.batch);
-      p.b = past ? __ffs(past) - 1 : P.batch;
-      p.base = __shfl_sync(kFullMask, upto - n, p.b & 31);
+      b = past ? __ffs(past) - 1 : P.batch;
+      base = __shfl_sync(kFullMask, upto - n, b & 31);
     } else {
-      total = total_blocks<KB>(P, lane, P.batch);
-      at = piece_begin(total, group, P.groups);
-      p = place_of<KB>(P, lane, at);
+      int64_t before, total;
+      count_blocks<KB>(P, lane, 0, before, total);
+      set_piece(P, total, group);
+      const Place p = place_of<KB>(P, lane, at);
+      b = p.b;
+      base = p.base;
     }
-    end = piece_begin(total, group + 1, P.groups);
-    b = p.b;
-    base = p.base;
+  }
+  __device__ void set_piece(const TreeParams& P, int64_t total, int group) {
+    const int groups = busy_groups(P, total);
+    at = group < groups ? piece_begin(total, group, groups) : 0;
+    end = group < groups ? piece_begin(total, group + 1, groups) : 0;
   }
   // the unit the piece is at, if it is not at its end
   __device__ bool unit(const TreeParams& P) {
@@ -390,7 +409,7 @@ struct Walk {
     length = length_of(P, b);
     cached = (length + KB - 1) / KB;
     per_unit = cached + draft_blocks<KB>(P);
-    h = (int)((at - base) / per_unit);
+    h = (int)quotient(at - base, per_unit);
     unit0 = base + (int64_t)h * per_unit;
     j0 = (int)(at - unit0);
     j1 = (int)min((int64_t)per_unit, end - unit0);
@@ -834,62 +853,65 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmKc, const __grid_constant__
 
 // ---- joining the partial results -----------------------------------------------------------
 
-// A warp per row of a unit that more than one group of CTAs worked on
-template <typename T, int DP, int RT, int KB>
+// WARPS warps per row of a unit that more than one group of CTAs worked on, each takes every WARPS-th group; eight warps a block.
+// Few rows with many partials (one token over a long cache: 32 rows of 34 partials, 22 us with a warp a row) need all of a block's
+// warps for a row, many rows have few partials each.
+template <typename T, int DP, int RT, int KB, int WARPS>
 __global__ void __launch_bounds__(256) tree_merge_kernel(const TreeParams P) {
   using namespace tree;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int rows = P.tokens * P.G, row = blockIdx.x * 8 + warp;
+  constexpr int C = DP / 32, ROWS = 8 / WARPS;
+  __shared__ __align__(16) float sums[WARPS > 1 ? 8 : 1][DP];
+  __shared__ float parts[WARPS > 1 ? 8 : 1];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, part = warp % WARPS;
+  const int rows = P.tokens * P.G, row = blockIdx.x * ROWS + warp / WARPS;
   const int b = blockIdx.y / P.kv_heads, h = blockIdx.y - b * P.kv_heads;
-  ptx::grid_wait();
-  if (row >= rows) return;
-  const int64_t total = total_blocks<KB>(P, lane, P.batch);
+  int64_t before, total;
+  count_blocks<KB>(P, lane, b, before, total);
+  const int groups = busy_groups(P, total);
   const int per_unit = cache_blocks<KB>(P, b) + draft_blocks<KB>(P);
-  const int64_t unit0 = total_blocks<KB>(P, lane, b) + (int64_t)h * per_unit;
-  // the group that has block x: the last whose piece begins at or before it
-  auto group_of = [&](int64_t x) { return (int)(((x + 1) * P.groups - 1) / total); };
-  const int g0 = group_of(unit0), g1 = group_of(unit0 + per_unit - 1);
-  if (g0 == g1) return;
-  const int tile = row / RT, local = row - tile * RT;
+  const int64_t unit0 = before + (int64_t)h * per_unit;
+  const int g0 = group_of(total, unit0, groups), g1 = group_of(total, unit0 + per_unit - 1, groups);
+  if (g0 == g1) return;                      // written as a whole (the same for all of a block)
+  ptx::grid_wait();
+  const bool there = row < rows;
+  const int tile = (there ? row : 0) / RT, local = (there ? row : 0) - tile * RT;
   auto slot_of = [&](int g) { return ((int64_t)g * P.tiles + tile) * 2 + (g == g0 ? 1 : 0); };
 
-  // two passes over the statistics: the largest maximum, then sums; lanes take groups side by side
   float top = -INFINITY;
-  for (int g = g0 + lane; g <= g1; g += 32) {
-    // a group without blocks has no piece, its place lies between those of its neighbours
-    if (piece_begin(total, g, P.groups) < piece_begin(total, g + 1, P.groups)) top = fmaxf(top, P.stats[slot_of(g) * RT + local].x);
-  }
+  for (int g = g0 + lane; g <= g1; g += 32) top = fmaxf(top, P.stats[slot_of(g) * RT + local].x);
   top = warp_max(top);
   const float ref = top == -INFINITY ? 0.f : top;
-  constexpr int C = DP / 32;
   float o[C], l = 0.f;
 #pragma unroll
   for (int c = 0; c < C; ++c) o[c] = 0.f;
-  for (int first = g0; first <= g1; first += 32) {
-    const int g = first + lane;
-    float w = 0.f;
-    const bool there = g <= g1 && piece_begin(total, g, P.groups) < piece_begin(total, g + 1, P.groups);
-    if (there) {
-      const float2 st = P.stats[slot_of(g) * RT + local];
-      w = exp2f(st.x - ref);
-      l += st.y * w;
-    }
-    unsigned todo = __ballot_sync(kFullMask, there);
-    while (todo) {
-      const int k = __ffs(todo) - 1;
-      todo &= todo - 1;
-      const float wk = __shfl_sync(kFullMask, w, k);
-      const float* src = P.partial + (slot_of(first + k) * RT + local) * DP + lane * C;
-      __align__(16) float v[C];
-      if constexpr (C == 4) *reinterpret_cast<float4*>(v) = *reinterpret_cast<const float4*>(src);
-      else *reinterpret_cast<float2*>(v) = *reinterpret_cast<const float2*>(src);
+#pragma unroll 4
+  for (int g = g0 + part; g <= g1; g += WARPS) {
+    const int64_t slot = slot_of(g);
+    const float2 st = P.stats[slot * RT + local];
+    const float w = exp2f(st.x - ref);
+    __align__(16) float v[C];
+    if constexpr (C == 4) *reinterpret_cast<float4*>(v) = *reinterpret_cast<const float4*>(P.partial + (slot * RT + local) * DP + lane * C);
+    else *reinterpret_cast<float2*>(v) = *reinterpret_cast<const float2*>(P.partial + (slot * RT + local) * DP + lane * C);
+    l += st.y * w;
 #pragma unroll
-      for (int c = 0; c < C; ++c) o[c] += v[c] * wk;
+    for (int c = 0; c < C; ++c) o[c] += v[c] * w;
+  }
+  if constexpr (WARPS > 1) {
+#pragma unroll
+    for (int c = 0; c < C; ++c) sums[warp][lane * C + c] = o[c];
+    if (lane == 0) parts[warp] = l;
+    __syncthreads();
+    if (part > 0) return;
+#pragma unroll
+    for (int k = 1; k < WARPS; ++k) {
+      l += parts[warp + k];
+#pragma unroll
+      for (int c = 0; c < C; ++c) o[c] += sums[warp + k][lane * C + c];
     }
   }
-  l = warp_sum(l);
+  if (!there) return;
   const int t = row / P.G, g = row - t * P.G;
-  const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
+  const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);      // a sum that is NaN stays NaN
   T* out = const_cast<T*>(row_of<T>(P.out, b, h * P.G + g, t));
 #pragma unroll
   for (int c = 0; c < C; ++c)
@@ -953,19 +975,28 @@ int64_t tree_workspace_bytes(const TreeParams& P, int dtype, int impl) { return 
   } while (0)
 
 // The merge starts while the last CTAs of the kernel before it are still at work, and waits for their results
+template <typename T, int DP, int RT, int KB, int WARPS>
+static cudaError_t launch_merge(const TreeParams& P, cudaStream_t stream) {
+  cudaLaunchConfig_t config = {};
+  constexpr int ROWS = 8 / WARPS;
+  config.gridDim = dim3((unsigned)(((int64_t)P.tokens * P.G + ROWS - 1) / ROWS), (unsigned)(P.batch * P.kv_heads));
+  config.blockDim = dim3(256);
+  config.stream = stream;
+  cudaLaunchAttribute overlap = {};
+  overlap.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  overlap.val.programmaticStreamSerializationAllowed = 1;
+  config.attrs = &overlap;
+  config.numAttrs = 1;
+  return cudaLaunchKernelEx(&config, tree_merge_kernel<T, DP, RT, KB, WARPS>, P);
+}
+
 template <typename T, int DP, int RT, int KB>
 static int run_merge(const TreeParams& P, const TreePlan& p, cudaStream_t stream) {
   if (p.groups > 1) {
-    cudaLaunchConfig_t config = {};
-    config.gridDim = dim3((unsigned)(((int64_t)P.tokens * P.G + 7) / 8), (unsigned)(P.batch * P.kv_heads));
-    config.blockDim = dim3(256);
-    config.stream = stream;
-    cudaLaunchAttribute overlap = {};
-    overlap.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    overlap.val.programmaticStreamSerializationAllowed = 1;
-    config.attrs = &overlap;
-    config.numAttrs = 1;
-    TREE_TRY(cudaLaunchKernelEx(&config, tree_merge_kernel<T, DP, RT, KB>, P));
+    // partials of a row if the sequences are alike: eight warps where there are more than four, as long as the rows are few
+    const int64_t units = (int64_t)P.batch * P.kv_heads;
+    const bool many = p.groups > 4 * units && units * P.tokens * P.G <= 8 * num_sms();
+    TREE_TRY((many ? launch_merge<T, DP, RT, KB, 8>(P, stream) : launch_merge<T, DP, RT, KB, 1>(P, stream)));
   }
   TREE_TRY(cudaGetLastError());
   count_launches(p.groups > 1 ? 2 : 1);
