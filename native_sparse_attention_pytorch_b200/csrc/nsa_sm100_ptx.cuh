@@ -255,6 +255,18 @@ __device__ __forceinline__ void tmem_st_bf16_row32(uint32_t taddr, const float (
         "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
       : "memory");
 }
+// The same for 16 probabilities
+__device__ __forceinline__ void tmem_st_bf16_row16(uint32_t taddr, const float (&x)[16]) {
+  uint32_t r[8];
+#pragma unroll
+  for (int c = 0; c < 8; ++c) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(x[2 * c], x[2 * c + 1]);
+    r[c] = *reinterpret_cast<const uint32_t*>(&h);
+  }
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
+               ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+               : "memory");
+}
 // D[tmem] (+)= A[tmem] * B[smem], A as written by tmem_st_bf16_row32; called by a converged warp, one lane issues.
 __device__ __forceinline__ void mma_bf16_tmem_a_elect(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc,
                                                       bool accumulate) {
@@ -331,21 +343,24 @@ __device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
   asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
 }
-// The largest of 32 values
-__device__ __forceinline__ float max32(const float (&s)[32]) {
+// The largest of N values
+template <int N>
+__device__ __forceinline__ float max_row(const float (&s)[N]) {
   float m[4] = {fmaxf(s[0], s[1]), fmaxf(s[2], s[3]), fmaxf(s[4], s[5]), fmaxf(s[6], s[7])};
 #pragma unroll
-  for (int x = 8; x < 32; x += 8)
+  for (int x = 8; x < N; x += 8)
 #pragma unroll
     for (int k = 0; k < 4; ++k) m[k] = max3(m[k], s[x + 2 * k], s[x + 2 * k + 1]);
   return fmaxf(max3(m[0], m[1], m[2]), m[3]);
 }
+__device__ __forceinline__ float max32(const float (&s)[32]) { return max_row<32>(s); }
 // s = 2^(s * scale2 - off) in place; the sum, in fp32 (four partial sums: values x with equal x % 4)
-__device__ __forceinline__ float exp_row32(float (&s)[32], float scale_log2, float off) {
+template <int N>
+__device__ __forceinline__ float exp_row(float (&s)[N], float scale_log2, float off) {
   const uint64_t scale2 = pack2(scale_log2, scale_log2), off2 = pack2(-off, -off);
   uint64_t l0 = 0ull, l1 = 0ull;
 #pragma unroll
-  for (int x = 0; x < 32; x += 4) {
+  for (int x = 0; x < N; x += 4) {
     unpack2(fma2(pack2(s[x], s[x + 1]), scale2, off2), s[x], s[x + 1]);
     unpack2(fma2(pack2(s[x + 2], s[x + 3]), scale2, off2), s[x + 2], s[x + 3]);
 #pragma unroll
@@ -358,6 +373,7 @@ __device__ __forceinline__ float exp_row32(float (&s)[32], float scale_log2, flo
   unpack2(l1, c, d);
   return (a + b) + (c + d);
 }
+__device__ __forceinline__ float exp_row32(float (&s)[32], float scale_log2, float off) { return exp_row<32>(s, scale_log2, off); }
 __device__ __forceinline__ void red_add_v4(float* addr, float a, float b, float c, float d) {
   asm volatile("red.global.add.v4.f32 [%0], {%1, %2, %3, %4};" ::"l"(addr), "f"(a), "f"(b), "f"(c), "f"(d) : "memory");
 }

@@ -341,8 +341,9 @@ __global__ void __launch_bounds__(tree_simt::kThreads, 2) tree_simt_kernel(const
 //   TMA warp        K and V blocks through a ring of slots (K, V, K, V, ...), across units and as far ahead as the ring holds
 //   mending warp    clears the rows of a V block that lie behind the sequence, and drafted values that are not finite
 //   MMA warp(s)     S = Q K^T, then O += P V with P from tensor memory; one per stream
-//   softmax warps   four per stream, a thread per row (the 32 lanes of tensor memory that a warp reaches): S from tensor memory,
-//                   maximum, exponentials, P back as bf16.  P is rounded (2^-9 on average a weight, as any bf16 tensor of
+//   softmax warps   S from tensor memory, maximum, exponentials, P back as bf16.  A warp reaches 32 lanes of tensor memory, 32 rows.
+//                   One stream: two threads per row, half of a block's keys each, which exchange maxima (one token over 4096 rows
+//                   10.1 us, with one thread 11.4).  Two streams: one thread (64 tokens over 65536 rows 502 us, with two 588).  P is rounded (2^-9 on average a weight, as any bf16 tensor of
 //                   weights would be); the sum adds the exponentials as they are.
 // The accumulator O stays in tensor memory.  It is rescaled lazily: a row keeps its reference maximum until a block exceeds it by
 // more than 2^8.
@@ -358,7 +359,8 @@ struct Shape {
   static constexpr uint32_t kTile = NC * 16384;                    // Q, K or V: 128 rows
   static constexpr int kSlots = (14 - STREAMS * NC) / NC;          // 14 tiles of 16 KB fit
   static constexpr uint32_t kBytes = (STREAMS + kSlots) * kTile;
-  static constexpr int kWarps = 4 * STREAMS + STREAMS + 2, kThreads = 32 * kWarps;
+  static constexpr int kHalves = STREAMS == 1 ? 2 : 1;             // threads of a row
+  static constexpr int kWarps = 4 * kHalves * STREAMS + STREAMS + 2, kThreads = 32 * kWarps;
 };
 constexpr int kMostSlots = 13, kAhead = 8;
 struct Bars {
@@ -439,23 +441,26 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmKc, const __grid_constant__
   using S = Shape<D, STREAMS>;
   using Walker = Walk<kKeys>;
   typedef __nv_bfloat16 T;
-  constexpr int NC = S::NC, kSlots = S::kSlots, LOOK = STREAMS == 1 ? 2 : 1, SOFT = 4 * STREAMS;
+  constexpr int NC = S::NC, kSlots = S::kSlots, LOOK = STREAMS == 1 ? 2 : 1, HALVES = S::kHalves, SOFT = 4 * HALVES * STREAMS;
   constexpr int RT = STREAMS * kRows / SPLIT;           // rows of the CTA's tile
-  constexpr int CW = kKeys / SPLIT;                     // keys of a thread in a block
+  constexpr int CW = kKeys / SPLIT / HALVES;                 // keys of a thread in a block
+  constexpr int CH = CW < 32 ? CW : 32, NCH = CW / CH;  // in pieces
   constexpr uint32_t kTile = S::kTile, tO = STREAMS == 1 ? 256 : 128, tP0 = STREAMS == 1 ? 384 : 0;
   extern __shared__ __align__(1024) uint8_t tree_tc_smem[];
   __shared__ int abort_flag;
   __shared__ uint32_t tmem_slot;
   __shared__ __align__(8) Bars bars;
   __shared__ volatile int odd_values[16];               // by unit: a drafted value is not finite
-  __shared__ float2 joined[SPLIT > 1 ? kRows : 1];      // maximum and sum of every copy of a row
+  // maxima, and sums at a unit's end, of the two threads of a row.  With one S buffer one place is enough: S of the next block comes
+  // behind P of this one, of all threads
+  __shared__ __align__(16) float xchg[HALVES > 1 ? STREAMS : 1][LOOK][2][HALVES > 1 ? kRows : 1];
 
   const uint32_t sQ0 = smem_u32(tree_tc_smem), sRing = sQ0 + STREAMS * kTile;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int tile = blockIdx.x % P.tiles, group = blockIdx.x / P.tiles;
   const int rows = P.tokens * P.G, row0 = tile * RT, here = min(RT, rows - row0);     // this tile's rows
   const int streams = STREAMS == 2 && here > kRows ? 2 : 1;
-  // softmax warps with rows, of a stream
+  // quarters of the tensor-core tile with rows, of a stream
   auto active = [&](int s) { return SPLIT > 1 ? 4 : max(0, min(4, (here - s * kRows + 31) / 32)); };
 
   if (tid == 0) {
@@ -466,10 +471,10 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmKc, const __grid_constant__
     }
     for (int i = 0; i < kAhead; ++i) mbar_init(smem_u32(&bars.ready[i]), 1);
     for (int s = 0; s < streams; ++s) {
-      mbar_init(smem_u32(&bars.q_full[s]), 32 * active(s));
+      mbar_init(smem_u32(&bars.q_full[s]), 32 * HALVES * active(s));
       for (int i = 0; i < LOOK; ++i) {
         mbar_init(smem_u32(&bars.s_full[s][i]), 1);
-        mbar_init(smem_u32(&bars.p_full[s][i]), 32 * active(s));
+        mbar_init(smem_u32(&bars.p_full[s][i]), 32 * HALVES * active(s));
         mbar_init(smem_u32(&bars.pv_done[s][i]), 1);
       }
       mbar_init(smem_u32(&bars.drain[s]), 1);
@@ -494,7 +499,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmKc, const __grid_constant__
 
   if (warp < SOFT) {
     // ------------------------------------------------------------------ softmax
-    const int s = warp >> 2, quarter = warp & 3;
+    const int s = warp / (4 * HALVES), quarter = warp & 3, half = HALVES > 1 ? (warp >> 2) & 1 : 0;
     const int part = quarter * SPLIT / 4;                                     // which keys of a block
     const int lane_row = quarter * 32 + lane;                                 // row of the tensor-core tile
     const int local = s * kRows + (SPLIT == 1 ? lane_row : lane_row % RT);    // row of the CTA's tile
@@ -503,14 +508,15 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmKc, const __grid_constant__
     const uint32_t tm_lane = tm + s * 256 + ((uint32_t)(quarter * 32) << 16);
     const float scale2 = P.scale * kLog2e;
     uint8_t* const region = tree_tc_smem + s * kTile;
-    auto stream_sync = [&]() { asm volatile("bar.sync %0, 128;" ::"r"(1 + s) : "memory"); };
+    auto pair_sync = [&]() { asm volatile("bar.sync %0, %1;" ::"r"(1 + s * 4 + quarter), "n"(32 * HALVES) : "memory"); };
+    auto stream_sync = [&]() { asm volatile("bar.sync %0, %1;" ::"r"(9 + s), "n"(128 * HALVES) : "memory"); };
     const bool working = s < streams && (SPLIT > 1 || local - lane < here);
     if (working && SPLIT > 1) {      // the keys that other copies take have weight zero here, always
       float zero[16];
 #pragma unroll
       for (int i = 0; i < 16; ++i) zero[i] = 0.f;
 #pragma unroll 1
-      for (int c = 0; c < 128; c += 16) tmem_st16(tm_lane + tP0 + c, zero);
+      for (int c = half * (128 / HALVES); c < (half + 1) * (128 / HALVES); c += 16) tmem_st16(tm_lane + tP0 + c, zero);
       tmem_st_wait();
     }
     uint32_t u = 0;
@@ -519,7 +525,8 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmKc, const __grid_constant__
       {
         const T* src = row_of<T>(P.q, walk.b, walk.h * P.G + g, t);
 #pragma unroll
-        for (int c = 0; c < D / 8; ++c) {
+        for (int cc = 0; cc < D / 8 / HALVES; ++cc) {
+          const int c = half * (D / 8 / HALVES) + cc;
           uint4 v = make_uint4(0, 0, 0, 0);
           if (valid && c * 8 < P.d) {
             if (q_vec) v = *reinterpret_cast<const uint4*>(src + c * 8);
@@ -535,42 +542,51 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmKc, const __grid_constant__
         fence_proxy_async_smem();
         mbar_arrive(smem_u32(&bars.q_full[s]));
       }
-      float m_ref = -INFINITY, l = 0.f;
+      float m_ref = -INFINITY, l = 0.f;         // l: of this thread's keys
       for (int j = walk.j0; j < walk.j1; ++j, ++u) {
         const uint32_t buf = u % LOOK, phase = (u / LOOK) & 1;
         const uint32_t tS = tm_lane + buf * 128;
         const uint32_t tP = STREAMS == 1 ? tm_lane + tP0 + buf * 64 : tm_lane;
         const bool draft = j >= walk.cached;
-        const int first = (draft ? j - walk.cached : j) * kKeys + part * CW, n = (draft ? P.tokens : walk.length) - first;
-        float x[CW / 32][32];
+        const int first = (draft ? j - walk.cached : j) * kKeys + (part * HALVES + half) * CW, n = (draft ? P.tokens : walk.length) - first;
+        float x[NCH][CH];
         mbar_wait_warp(smem_u32(&bars.s_full[s][buf]), phase, &abort_flag);
         tc_fence_after_sync();
 #pragma unroll
-        for (int k = 0; k < CW / 32; ++k) tmem_ld32(tS + part * CW + k * 32, x[k]);
+        for (int k = 0; k < NCH; ++k) {
+          if constexpr (CH == 32) tmem_ld32(tS + (part * HALVES + half) * CW + k * 32, x[k]);
+          else tmem_ld16(tS + (part * HALVES + half) * CW, x[k]);
+        }
         tmem_ld_wait();
         if (draft) {
 #pragma unroll
-          for (int k = 0; k < CW / 32; ++k) {
+          for (int k = 0; k < NCH; ++k) {
             uint32_t seen = 0;
             if (valid) {
 #pragma unroll 8
-              for (int i = 0; i < 32; ++i)
-                if (k * 32 + i < n && sees(P, walk.b, t, first + k * 32 + i)) seen |= 1u << i;
+              for (int i = 0; i < CH; ++i)
+                if (k * CH + i < n && sees(P, walk.b, t, first + k * CH + i)) seen |= 1u << i;
             }
 #pragma unroll
-            for (int i = 0; i < 32; ++i)
+            for (int i = 0; i < CH; ++i)
               if (!(seen >> i & 1)) x[k][i] = -INFINITY;
           }
         } else if (n < CW) {
 #pragma unroll
-          for (int k = 0; k < CW / 32; ++k)
+          for (int k = 0; k < NCH; ++k)
 #pragma unroll
-            for (int i = 0; i < 32; ++i)
-              if (k * 32 + i >= n) x[k][i] = -INFINITY;
+            for (int i = 0; i < CH; ++i)
+              if (k * CH + i >= n) x[k][i] = -INFINITY;
         }
-        float m = max32(x[0]);
+        float m = max_row<CH>(x[0]);
 #pragma unroll
-        for (int k = 1; k < CW / 32; ++k) m = fmaxf(m, max32(x[k]));
+        for (int k = 1; k < NCH; ++k) m = fmaxf(m, max_row<CH>(x[k]));
+        // the row's maximum over both threads; behind the barrier both have read their S columns
+        if (HALVES > 1) {
+          xchg[s][buf][half][lane_row] = m;
+          pair_sync();
+          m = fmaxf(m, xchg[s][buf][half ^ 1][lane_row]);
+        }
         const float m2 = m * scale2;              // -inf: nothing seen
         bool need = false;
         float alpha = 1.f;
@@ -587,7 +603,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmKc, const __grid_constant__
           if (LOOK == 2) mbar_wait_warp(smem_u32(&bars.pv_done[s][(u - 1) % LOOK]), ((u - 1) / LOOK) & 1, &abort_flag);
           tc_fence_after_sync();
 #pragma unroll 1
-          for (int c = 0; c < D; c += 16) {
+          for (int c = half * (D / HALVES); c < (half + 1) * (D / HALVES); c += 16) {
             float o[16];
             tmem_ld16(tm_lane + tO + c, o);
             tmem_ld_wait();
@@ -599,9 +615,10 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmKc, const __grid_constant__
         }
         const float ref = m_ref == -INFINITY ? 0.f : m_ref;     // -inf - -inf must not be formed
 #pragma unroll
-        for (int k = 0; k < CW / 32; ++k) {
-          l += exp_row32(x[k], scale2, ref);
-          tmem_st_bf16_row32(tP + part * (CW / 2) + k * 16, x[k]);
+        for (int k = 0; k < NCH; ++k) {
+          l += exp_row<CH>(x[k], scale2, ref);
+          if constexpr (CH == 32) tmem_st_bf16_row32(tP + (part * HALVES + half) * (CW / 2) + k * 16, x[k]);
+          else tmem_st_bf16_row16(tP + (part * HALVES + half) * (CW / 2), x[k]);
         }
         tmem_st_wait();
         tc_fence_before_sync();
@@ -610,6 +627,11 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmKc, const __grid_constant__
       // the unit's end: O of this CTA's blocks, complete or a partial result
       mbar_wait_warp(smem_u32(&bars.pv_done[s][(u - 1) % LOOK]), ((u - 1) / LOOK) & 1, &abort_flag);
       tc_fence_after_sync();
+      if (HALVES > 1) {                           // (all threads have given P of the last block, and so read its maxima)
+        xchg[s][u % LOOK][half][lane_row] = l;
+        pair_sync();
+        l += xchg[s][u % LOOK][half ^ 1][lane_row];
+      }
       const bool whole = walk.j0 == 0 && walk.j1 == walk.per_unit;
       const int64_t slot = (int64_t)blockIdx.x * 2 + (walk.j0 == 0 ? 1 : 0);
       const int u0 = max(0, walk.j0 - walk.cached) * kKeys, u1 = min(P.tokens, (walk.j1 - walk.cached) * kKeys);
@@ -651,7 +673,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmKc, const __grid_constant__
       };
       if constexpr (SPLIT == 1) {
 #pragma unroll 1
-        for (int c = 0; c < D; c += 32) {
+        for (int c = half * (D / HALVES); c < (half + 1) * (D / HALVES); c += 32) {
           float o[32];
           tmem_ld32(tm_lane + tO + c, o);
           tmem_ld_wait();
@@ -660,11 +682,13 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmKc, const __grid_constant__
             for (int k = 0; k < 4; ++k) store8(local, t, walk.h * P.G + g, c + 8 * k, l, o + 8 * k);
           __syncwarp();
         }
-        if (valid) store_stats(local, t, walk.h * P.G + g, m_ref, l);
+        if (valid && half == 0) store_stats(local, t, walk.h * P.G + g, m_ref, l);
+        if (HALVES > 1) pair_sync();        // both have read the sums: the next unit's first block may write the same place
       } else {
         // join the copies: the upper half of them leaves its rows in Q's place, the lower half adds its own, then all threads
         // take rows apart
-        joined[lane_row] = make_float2(m_ref, l);
+        float2* const joined = reinterpret_cast<float2*>(&xchg[s][(u + 1) % LOOK][0][0]);    // maximum and sum of every copy of a row
+        if (half == 0) joined[lane_row] = make_float2(m_ref, l);
         stream_sync();
         float top = -INFINITY, sum = 0.f;
 #pragma unroll
@@ -677,7 +701,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmKc, const __grid_constant__
         auto piece = [&](int k, int r, int c4) { return reinterpret_cast<float4*>(region + (size_t)(k * RT + r) * (D * 4)) + (c4 ^ (r & 7)); };
         if (part >= SPLIT / 2) {
 #pragma unroll 1
-          for (int c = 0; c < D; c += 16) {
+          for (int c = half * (D / HALVES); c < (half + 1) * (D / HALVES); c += 16) {
             float o[16];
             tmem_ld16(tm_lane + tO + c, o);
             tmem_ld_wait();
@@ -689,7 +713,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmKc, const __grid_constant__
         stream_sync();
         if (part < SPLIT / 2) {
 #pragma unroll 1
-          for (int c = 0; c < D; c += 16) {
+          for (int c = half * (D / HALVES); c < (half + 1) * (D / HALVES); c += 16) {
             float o[16];
             tmem_ld16(tm_lane + tO + c, o);
             tmem_ld_wait();
@@ -702,11 +726,11 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmKc, const __grid_constant__
             }
           }
         }
-        if (quarter == 0 || (SPLIT == 2 && quarter == 1)) {
+        if (half == 0 && (quarter == 0 || (SPLIT == 2 && quarter == 1))) {
           if (valid) store_stats(local, t, walk.h * P.G + g, top, sum);
         }
         stream_sync();
-        for (int e = lane_row; e < here * (D / 8); e += 128) {
+        for (int e = half * 128 + lane_row; e < here * (D / 8); e += 128 * HALVES) {
           const int r = e / (D / 8), c = (e - r * (D / 8)) * 8, rr = row0 + r, token = rr / P.G;
           float o[8], total = 0.f, high = -INFINITY;
 #pragma unroll
