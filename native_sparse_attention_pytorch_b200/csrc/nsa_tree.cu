@@ -337,7 +337,7 @@ __global__ void __launch_bounds__(tree_simt::kThreads, 2) tree_simt_kernel(const
 
 // ---- bf16, on the tensor cores ---------------------------------------------------------------
 
-// A persistent CTA per SM goes through its piece of the key blocks (128 keys):
+// A persistent CTA per SM goes through its piece of the key blocks (128 keys, with two streams 64):
 //   TMA warp        K and V blocks through a ring of slots (K, V, K, V, ...), across units and as far ahead as the ring holds
 //   mending warp    clears the rows of a V block that lie behind the sequence, and drafted values that are not finite
 //   MMA warp(s)     S = Q K^T, then O += P V with P from tensor memory; one per stream
@@ -350,19 +350,23 @@ __global__ void __launch_bounds__(tree_simt::kThreads, 2) tree_simt_kernel(const
 // SPLIT.  A tensor-core tile has 128 rows however few there are.  Up to 32 rows are written four times over, and warp w takes keys
 // 32 w .. 32 w + 31 of every block for its copy (its P has zeros elsewhere): a quarter of the exponentials a thread, at no cost in
 // products.  Up to 64 rows twice, for halves.  The copies' results are joined in shared memory (in Q's place) where a unit ends.
-// STREAMS.  Above 128 rows two tiles share the K and V blocks; the softmax of one runs under the products of the other.
+// STREAMS.  Above 128 rows two tiles share the K and V blocks; the softmax of one runs under the products of the other.  Blocks of 64
+// keys, so that tensor memory holds two S buffers of either beside both O: with blocks of 128 and one buffer, S of the next block
+// waited for the products of this one, which waited for its softmax (3800 cycles a block and pair of tiles, 2050 of them products).
 namespace tree_tc {
-constexpr int kKeys = 128, kRows = 128;
+constexpr int kRows = 128;
+constexpr int keys(int streams) { return streams == 1 ? 128 : 64; }     // of a block
 template <int D, int STREAMS>
 struct Shape {
+  static constexpr int KK = keys(STREAMS);
   static constexpr int NC = D / 64;                                // 64-column subtiles of a row
-  static constexpr uint32_t kTile = NC * 16384;                    // Q, K or V: 128 rows
-  static constexpr int kSlots = (14 - STREAMS * NC) / NC;          // 14 tiles of 16 KB fit
-  static constexpr uint32_t kBytes = (STREAMS + kSlots) * kTile;
+  static constexpr uint32_t kTileQ = NC * 16384, kSub = KK * 128, kTile = NC * kSub;
+  static constexpr int kSlots = (14 * 16384 - STREAMS * kTileQ) / kTile;
+  static constexpr uint32_t kBytes = STREAMS * kTileQ + kSlots * kTile;
   static constexpr int kHalves = STREAMS == 1 ? 2 : 1;             // threads of a row
   static constexpr int kWarps = 4 * kHalves * STREAMS + STREAMS + 2, kThreads = 32 * kWarps;
 };
-constexpr int kMostSlots = 13, kAhead = 8;
+constexpr int kMostSlots = 24, kAhead = 16;
 struct Bars {
   uint64_t full[kMostSlots], free[kMostSlots];
   uint64_t ready[kAhead];         // V blocks, by their number: the mending warp is never this many ahead of the products
@@ -439,23 +443,25 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmKc, const __grid_constant__
   using namespace tree;
   using namespace tree_tc;
   using S = Shape<D, STREAMS>;
+  constexpr int kKeys = S::KK, LOOK = 2;                // keys of a block; S is computed two blocks ahead of P V
   using Walker = Walk<kKeys>;
   typedef __nv_bfloat16 T;
-  constexpr int NC = S::NC, kSlots = S::kSlots, LOOK = STREAMS == 1 ? 2 : 1, HALVES = S::kHalves, SOFT = 4 * HALVES * STREAMS;
+  constexpr int NC = S::NC, kSlots = S::kSlots, HALVES = S::kHalves, SOFT = 4 * HALVES * STREAMS;
   constexpr int RT = STREAMS * kRows / SPLIT;           // rows of the CTA's tile
   constexpr int CW = kKeys / SPLIT / HALVES;                 // keys of a thread in a block
   constexpr int CH = CW < 32 ? CW : 32, NCH = CW / CH;  // in pieces
-  constexpr uint32_t kTile = S::kTile, tO = STREAMS == 1 ? 256 : 128, tP0 = STREAMS == 1 ? 384 : 0;
+  constexpr uint32_t kTile = S::kTile, kTileQ = S::kTileQ, kSub = S::kSub;
+  // tensor memory of a stream: two S buffers, O behind them; P over the S it came from, or (copies) in a place of its own
+  constexpr uint32_t tO = 2 * kKeys, tP0 = STREAMS == 1 ? 384 : 0, tPstep = STREAMS == 1 ? 64 : kKeys;
   extern __shared__ __align__(1024) uint8_t tree_tc_smem[];
   __shared__ int abort_flag;
   __shared__ uint32_t tmem_slot;
   __shared__ __align__(8) Bars bars;
   __shared__ volatile int odd_values[16];               // by unit: a drafted value is not finite
-  // maxima, and sums at a unit's end, of the two threads of a row.  With one S buffer one place is enough: S of the next block comes
-  // behind P of this one, of all threads
+  // maxima, and sums at a unit's end, of the two threads of a row
   __shared__ __align__(16) float xchg[HALVES > 1 ? STREAMS : 1][LOOK][2][HALVES > 1 ? kRows : 1];
 
-  const uint32_t sQ0 = smem_u32(tree_tc_smem), sRing = sQ0 + STREAMS * kTile;
+  const uint32_t sQ0 = smem_u32(tree_tc_smem), sRing = sQ0 + STREAMS * kTileQ;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int tile = blockIdx.x % P.tiles, group = blockIdx.x / P.tiles;
   const int rows = P.tokens * P.G, row0 = tile * RT, here = min(RT, rows - row0);     // this tile's rows
@@ -507,7 +513,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmKc, const __grid_constant__
     const bool valid = local < here;
     const uint32_t tm_lane = tm + s * 256 + ((uint32_t)(quarter * 32) << 16);
     const float scale2 = P.scale * kLog2e;
-    uint8_t* const region = tree_tc_smem + s * kTile;
+    uint8_t* const region = tree_tc_smem + s * kTileQ;
     auto pair_sync = [&]() { asm volatile("bar.sync %0, %1;" ::"r"(1 + s * 4 + quarter), "n"(32 * HALVES) : "memory"); };
     auto stream_sync = [&]() { asm volatile("bar.sync %0, %1;" ::"r"(9 + s), "n"(128 * HALVES) : "memory"); };
     const bool working = s < streams && (SPLIT > 1 || local - lane < here);
@@ -537,7 +543,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmKc, const __grid_constant__
               v = *reinterpret_cast<const uint4*>(x);
             }
           }
-          sts_v4(sQ0 + s * kTile + (c / 8) * 16384 + sw128_offset(lane_row, c & 7), v);
+          sts_v4(sQ0 + s * kTileQ + (c / 8) * 16384 + sw128_offset(lane_row, c & 7), v);
         }
         fence_proxy_async_smem();
         mbar_arrive(smem_u32(&bars.q_full[s]));
@@ -545,8 +551,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmKc, const __grid_constant__
       float m_ref = -INFINITY, l = 0.f;         // l: of this thread's keys
       for (int j = walk.j0; j < walk.j1; ++j, ++u) {
         const uint32_t buf = u % LOOK, phase = (u / LOOK) & 1;
-        const uint32_t tS = tm_lane + buf * 128;
-        const uint32_t tP = STREAMS == 1 ? tm_lane + tP0 + buf * 64 : tm_lane;
+        const uint32_t tS = tm_lane + buf * kKeys, tP = tm_lane + tP0 + buf * tPstep;
         const bool draft = j >= walk.cached;
         const int first = (draft ? j - walk.cached : j) * kKeys + (part * HALVES + half) * CW, n = (draft ? P.tokens : walk.length) - first;
         float x[NCH][CH];
@@ -599,8 +604,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmKc, const __grid_constant__
           need = true;
         }
         if (j > walk.j0 && __any_sync(kFullMask, need)) {
-          // with one S buffer the products of the block before are complete: S of this one came behind them
-          if (LOOK == 2) mbar_wait_warp(smem_u32(&bars.pv_done[s][(u - 1) % LOOK]), ((u - 1) / LOOK) & 1, &abort_flag);
+          mbar_wait_warp(smem_u32(&bars.pv_done[s][(u - 1) % LOOK]), ((u - 1) / LOOK) & 1, &abort_flag);
           tc_fence_after_sync();
 #pragma unroll 1
           for (int c = half * (D / HALVES); c < (half + 1) * (D / HALVES); c += 16) {
@@ -759,7 +763,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmKc, const __grid_constant__
       constexpr uint32_t idS = instr_desc_bf16(128, kKeys, false, false);
       constexpr uint32_t idO = instr_desc_bf16(128, D, false, true);
       const uint32_t ts = tm + s * 256;
-      const uint64_t dQ = smem_desc_sw128(sQ0 + s * kTile, 16);
+      const uint64_t dQ = smem_desc_sw128(sQ0 + s * kTileQ, 16);
       uint32_t u = 0, su = 0, units = 0;      // blocks whose P V, whose S has been issued
       auto issue_s = [&]() {
         const uint32_t slot = 2 * su % kSlots, round = 2 * su / kSlots;
@@ -769,8 +773,8 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmKc, const __grid_constant__
         const uint64_t dK = smem_desc_sw128(sRing + slot * kTile, 16);
 #pragma unroll
         for (int k = 0; k < D / 16; ++k)
-          mma_bf16_elect(ts + (su % LOOK) * 128, desc_advance(dQ, (k / 4) * 16384 + (k % 4) * 32),
-                         desc_advance(dK, (k / 4) * 16384 + (k % 4) * 32), idS, k > 0);
+          mma_bf16_elect(ts + (su % LOOK) * kKeys, desc_advance(dQ, (k / 4) * 16384 + (k % 4) * 32),
+                         desc_advance(dK, (k / 4) * kSub + (k % 4) * 32), idS, k > 0);
         mma_commit_elect(smem_u32(&bars.s_full[s][su % LOOK]));
         mma_commit_elect(smem_u32(&bars.free[slot]));
         ++su;
@@ -785,8 +789,8 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmKc, const __grid_constant__
           mbar_wait_bounded(smem_u32(&bars.p_full[s][u % LOOK]), (u / LOOK) & 1, &abort_flag);
           __syncwarp();
           tc_fence_after_sync();
-          const uint64_t dV = smem_desc_sw128(sRing + slot * kTile, 16384);
-          const uint32_t tP = STREAMS == 1 ? ts + tP0 + (u % LOOK) * 64 : ts;
+          const uint64_t dV = smem_desc_sw128(sRing + slot * kTile, kSub);
+          const uint32_t tP = ts + tP0 + (u % LOOK) * tPstep;
 #pragma unroll
           for (int k = 0; k < kKeys / 16; ++k) mma_bf16_tmem_a_elect(ts + tO, tP + k * 8, desc_advance(dV, k * 2048), idO, t > 0 || k > 0);
           mma_commit_elect(smem_u32(&bars.pv_done[s][u % LOOK]));
@@ -815,7 +819,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmKc, const __grid_constant__
             const int hh = walk.h * (draft ? (v ? A.v_h : A.k_h) : (v ? A.vc_h : A.kc_h));
             mbar_arrive_expect_tx(smem_u32(&bars.full[slot]), kTile);
 #pragma unroll
-            for (int c = 0; c < NC; ++c) tma_load_4d(sRing + slot * kTile + c * 16384, map, smem_u32(&bars.full[slot]), c * 64, first, hh, bb);
+            for (int c = 0; c < NC; ++c) tma_load_4d(sRing + slot * kTile + c * kSub, map, smem_u32(&bars.full[slot]), c * 64, first, hh, bb);
           }
           __syncwarp();
         }
@@ -840,10 +844,10 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmKc, const __grid_constant__
         if (draft || n < kKeys) {
           if (!draft)       // behind the drafted rows the tile is zero as loaded
             for (int e = lane; e < (kKeys - n) * 8 * NC; e += 32)
-              sts_v4(at + (e & (NC - 1)) * 16384 + sw128_offset(n + (e / NC) / 8, (e / NC) & 7), make_uint4(0, 0, 0, 0));
+              sts_v4(at + (e & (NC - 1)) * kSub + sw128_offset(n + (e / NC) / 8, (e / NC) & 7), make_uint4(0, 0, 0, 0));
           else
             for (int e = lane; e < n * 8 * NC; e += 32) {
-              const uint32_t p = at + (e & (NC - 1)) * 16384 + sw128_offset((e / NC) / 8, (e / NC) & 7);
+              const uint32_t p = at + (e & (NC - 1)) * kSub + sw128_offset((e / NC) / 8, (e / NC) & 7);
               const uint4 v = lds_v4(p);
               uint32_t w[4] = {v.x, v.y, v.z, v.w};
               bool bad = false;
@@ -973,7 +977,7 @@ static TreePlan plan_tree(const TreeParams& P, int dtype, int impl) {
   int64_t ctas = num_sms();
   if (p.tensor_cores) {
     p.RT = rows <= 32 ? 32 : rows <= 64 ? 64 : rows <= 128 ? 128 : 256;
-    p.KB = tree_tc::kKeys;
+    p.KB = tree_tc::keys(p.RT <= 128 ? 1 : 2);
   } else {
     p.RT = rows <= 8 ? 8 : 32;
     p.KB = tree_simt::kKeys;
@@ -1044,15 +1048,15 @@ static int run_simt_typed(const TreeParams& P, const TreePlan& p, cudaStream_t s
   return p.RT == 8 ? run_simt<T, 128, 8>(P, p, stream) : run_simt<T, 128, 32>(P, p, stream);
 }
 
-// Boxes of 64 features x 128 rows of one head.  An axis of one entry, or of stride zero, is one entry in the map; `step_b` and
+// Boxes of 64 features x `rows` rows of one head.  An axis of one entry, or of stride zero, is one entry in the map; `step_b` and
 // `step_h` say whether coordinates move along it.
-static int make_tree_map(CUtensorMap* map, const RowView& r, int B, int H, int64_t N, int d, int* step_b, int* step_h) {
+static int make_tree_map(CUtensorMap* map, const RowView& r, int B, int H, int64_t N, int d, int rows, int* step_b, int* step_h) {
   *step_b = B > 1 && r.sb > 0;
   *step_h = H > 1 && r.sh > 0;
   const uint64_t row = N > 1 ? (uint64_t)r.sn * 2 : (uint64_t)d * 2;
   const uint64_t dims[4] = {(uint64_t)d, (uint64_t)N, (uint64_t)(*step_h ? H : 1), (uint64_t)(*step_b ? B : 1)};
   const uint64_t strides[3] = {row, *step_h ? (uint64_t)r.sh * 2 : row, *step_b ? (uint64_t)r.sb * 2 : row};
-  const uint32_t box[4] = {64, tree_tc::kKeys, 1, 1};
+  const uint32_t box[4] = {64, (uint32_t)rows, 1, 1};
   return encode_bf16_tiles(map, r.p, dims, strides, box);
 }
 
@@ -1061,16 +1065,16 @@ static int run_tc(const TreeParams& P, const TreePlan& p, cudaStream_t stream) {
   using S = tree_tc::Shape<D, STREAMS>;
   CUtensorMap tmKc, tmVc, tmK, tmV;
   TreeAxes A = {};
-  int rc = make_tree_map(&tmK, P.k, P.batch, P.kv_heads, P.tokens, P.d, &A.k_b, &A.k_h);
-  if (rc == NSA_OK) rc = make_tree_map(&tmV, P.v, P.batch, P.kv_heads, P.tokens, P.d, &A.v_b, &A.v_h);
+  int rc = make_tree_map(&tmK, P.k, P.batch, P.kv_heads, P.tokens, P.d, S::KK, &A.k_b, &A.k_h);
+  if (rc == NSA_OK) rc = make_tree_map(&tmV, P.v, P.batch, P.kv_heads, P.tokens, P.d, S::KK, &A.v_b, &A.v_h);
   tmKc = tmK; tmVc = tmV;                 // an empty cache is never looked at
-  if (rc == NSA_OK && P.capacity > 0) rc = make_tree_map(&tmKc, P.kc, P.batch, P.kv_heads, P.capacity, P.d, &A.kc_b, &A.kc_h);
-  if (rc == NSA_OK && P.capacity > 0) rc = make_tree_map(&tmVc, P.vc, P.batch, P.kv_heads, P.capacity, P.d, &A.vc_b, &A.vc_h);
+  if (rc == NSA_OK && P.capacity > 0) rc = make_tree_map(&tmKc, P.kc, P.batch, P.kv_heads, P.capacity, P.d, S::KK, &A.kc_b, &A.kc_h);
+  if (rc == NSA_OK && P.capacity > 0) rc = make_tree_map(&tmVc, P.vc, P.batch, P.kv_heads, P.capacity, P.d, S::KK, &A.vc_b, &A.vc_h);
   if (rc != NSA_OK) return rc;
   const int q_vec = (reinterpret_cast<uintptr_t>(P.q.p) & 15u) == 0 && P.q.sb % 8 == 0 && P.q.sh % 8 == 0 && P.q.sn % 8 == 0;
   TREE_TRY((allow_shared_memory<tree_tc_kernel<D, STREAMS, SPLIT>>()));
   tree_tc_kernel<D, STREAMS, SPLIT><<<(unsigned)(p.groups * p.tiles), S::kThreads, S::kBytes, stream>>>(tmKc, tmVc, tmK, tmV, P, A, q_vec);
-  return run_merge<__nv_bfloat16, D, STREAMS * tree_tc::kRows / SPLIT, tree_tc::kKeys>(P, p, stream);
+  return run_merge<__nv_bfloat16, D, STREAMS * tree_tc::kRows / SPLIT, S::KK>(P, p, stream);
 }
 
 template <int D>
