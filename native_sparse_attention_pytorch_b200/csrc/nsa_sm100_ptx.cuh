@@ -255,18 +255,6 @@ __device__ __forceinline__ void tmem_st_bf16_row32(uint32_t taddr, const float (
         "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
       : "memory");
 }
-// The same for 16 probabilities
-__device__ __forceinline__ void tmem_st_bf16_row16(uint32_t taddr, const float (&x)[16]) {
-  uint32_t r[8];
-#pragma unroll
-  for (int c = 0; c < 8; ++c) {
-    const __nv_bfloat162 h = __floats2bfloat162_rn(x[2 * c], x[2 * c + 1]);
-    r[c] = *reinterpret_cast<const uint32_t*>(&h);
-  }
-  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
-               ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
-               : "memory");
-}
 // D[tmem] (+)= A[tmem] * B[smem], A as written by tmem_st_bf16_row32; called by a converged warp, one lane issues.
 __device__ __forceinline__ void mma_bf16_tmem_a_elect(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc,
                                                       bool accumulate) {
@@ -343,6 +331,11 @@ __device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
   asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
 }
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
 // The largest of N values
 template <int N>
 __device__ __forceinline__ float max_row(const float (&s)[N]) {
@@ -355,12 +348,11 @@ __device__ __forceinline__ float max_row(const float (&s)[N]) {
 }
 __device__ __forceinline__ float max32(const float (&s)[32]) { return max_row<32>(s); }
 // s = 2^(s * scale2 - off) in place; the sum, in fp32 (four partial sums: values x with equal x % 4)
-template <int N>
-__device__ __forceinline__ float exp_row(float (&s)[N], float scale_log2, float off) {
+__device__ __forceinline__ float exp_row32(float (&s)[32], float scale_log2, float off) {
   const uint64_t scale2 = pack2(scale_log2, scale_log2), off2 = pack2(-off, -off);
   uint64_t l0 = 0ull, l1 = 0ull;
 #pragma unroll
-  for (int x = 0; x < N; x += 4) {
+  for (int x = 0; x < 32; x += 4) {
     unpack2(fma2(pack2(s[x], s[x + 1]), scale2, off2), s[x], s[x + 1]);
     unpack2(fma2(pack2(s[x + 2], s[x + 3]), scale2, off2), s[x + 2], s[x + 3]);
 #pragma unroll
@@ -373,7 +365,67 @@ __device__ __forceinline__ float exp_row(float (&s)[N], float scale_log2, float 
   unpack2(l1, c, d);
   return (a + b) + (c + d);
 }
-__device__ __forceinline__ float exp_row32(float (&s)[32], float scale_log2, float off) { return exp_row<32>(s, scale_log2, off); }
+// The same, rounded to bf16 pairs as the A operand in tensor memory holds them (element 2c in the low half of r[c]).  Sums and
+// roundings follow the exponentials at a distance of eight values: a warp issues in order, and what waits for an exponential holds
+// up the next.  SHARE of every 16 values go to the multiplying units instead of the exponential unit, which takes eight cycles for a
+// warp's 32: 2^x = 2^n 2^f with n the nearest whole number (by adding 1.5 * 2^23, + 127 so that the low bits are n's exponent) and
+// |f| <= 1/2, 2^f by its polynomial of degree 4 with the least relative error (2.7e-6 in fp32; found by the Remez exchange).  Below
+// 2^-126 a value counts as that (so SHARE > 0 is for rows without masked logits); NaN stays.
+template <int N, int SHARE>
+__device__ __forceinline__ float exp_pack_row(float (&s)[N], float scale_log2, float off, uint32_t (&r)[N / 2]) {
+  constexpr float kMagic = 12582912.f + 127.f;
+  constexpr int kBehind = 8;
+  const uint64_t scale2 = pack2(scale_log2, scale_log2), off2 = pack2(-off, -off);
+  const uint64_t magic = pack2(kMagic, kMagic), less = pack2(-kMagic, -kMagic), minus = pack2(-1.f, -1.f);
+  const uint64_t c0 = pack2(0.9999992847442627f, 0.9999992847442627f), c1 = pack2(0.6931217908859253f, 0.6931217908859253f),
+                 c2 = pack2(0.240247443318367f, 0.240247443318367f), c3 = pack2(0.05591785907745361f, 0.05591785907745361f),
+                 c4 = pack2(0.009570102207362652f, 0.009570102207362652f);
+  uint64_t l0 = 0ull, l1 = 0ull;
+#pragma unroll
+  for (int x = 0; x < N; x += 2) unpack2(fma2(pack2(s[x], s[x + 1]), scale2, off2), s[x], s[x + 1]);
+#pragma unroll
+  for (int x = 0; x < N + kBehind; x += 2) {
+    if (x < N) {
+      if (x % 16 < 16 - SHARE) {
+        s[x] = ex2(s[x]);
+        s[x + 1] = ex2(s[x + 1]);
+      } else {
+        float a, b;
+        asm("max.NaN.f32 %0, %1, 0fC2FC0000;" : "=f"(a) : "f"(s[x]));          // -126
+        asm("max.NaN.f32 %0, %1, 0fC2FC0000;" : "=f"(b) : "f"(s[x + 1]));
+        const uint64_t y = pack2(a, b), t = add2(y, magic), f = fma2(add2(t, less), minus, y);
+        const uint64_t p = fma2(fma2(fma2(fma2(c4, f, c3), f, c2), f, c1), f, c0);
+        float ta, tb;
+        unpack2(t, ta, tb);
+        unpack2(mul2(p, pack2(__uint_as_float(__float_as_uint(ta) << 23), __uint_as_float(__float_as_uint(tb) << 23))), s[x], s[x + 1]);
+      }
+    }
+    if (x >= kBehind) {
+      const int y = x - kBehind;
+      if (y % 4 == 0) l0 = add2(l0, pack2(s[y], s[y + 1]));
+      else l1 = add2(l1, pack2(s[y], s[y + 1]));
+      r[y / 2] = pack_bf16(s[y], s[y + 1]);
+    }
+  }
+  float a, b, c, d;
+  unpack2(l0, a, b);
+  unpack2(l1, c, d);
+  return (a + b) + (c + d);
+}
+// 16 or 8 columns of such pairs of the lane's row
+__device__ __forceinline__ void tmem_st_words(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
+      ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
+        "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st_words(uint32_t taddr, const uint32_t (&r)[8]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
+               ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+               : "memory");
+}
 __device__ __forceinline__ void red_add_v4(float* addr, float a, float b, float c, float d) {
   asm volatile("red.global.add.v4.f32 [%0], {%1, %2, %3, %4};" ::"l"(addr), "f"(a), "f"(b), "f"(c), "f"(d) : "memory");
 }
@@ -382,11 +434,6 @@ __device__ __forceinline__ void sts_v4(uint32_t addr, uint4 v) {
                : "memory");
 }
 __device__ __forceinline__ void sts_u32(uint32_t addr, uint32_t v) { asm volatile("st.shared.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory"); }
-__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
-  uint32_t r;
-  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-  return r;
-}
 
 __device__ __forceinline__ uint2 lds_v2(uint32_t addr) {
   uint2 v;

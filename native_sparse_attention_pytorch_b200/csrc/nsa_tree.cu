@@ -353,6 +353,10 @@ __global__ void __launch_bounds__(tree_simt::kThreads, 2) tree_simt_kernel(const
 // STREAMS.  Above 128 rows two tiles share the K and V blocks; the softmax of one runs under the products of the other.  Blocks of 64
 // keys, so that tensor memory holds two S buffers of either beside both O: with blocks of 128 and one buffer, S of the next block
 // waited for the products of this one, which waited for its softmax (3800 cycles a block and pair of tiles, 2050 of them products).
+#ifndef TREE_SHARE
+#define TREE_SHARE 0
+#define TREE_TURNS 1
+#endif
 namespace tree_tc {
 constexpr int kRows = 128;
 constexpr int keys(int streams) { return streams == 1 ? 128 : 64; }     // of a block
@@ -382,9 +386,10 @@ struct Walk {
   int b, h, length, cached, per_unit, j0, j1;
   int64_t base, at, end, unit0;
   // by a whole warp
+  __device__ void ask(const TreeParams& P, int lane) { length = lane < P.batch ? length_of(P, lane) : 0; }
   __device__ void begin(const TreeParams& P, int lane, int group) {
     if (P.batch <= 32) {                  // one look at the lengths
-      const int64_t n = lane < P.batch ? ((int64_t)cache_blocks<KB>(P, lane) + draft_blocks<KB>(P)) * P.kv_heads : 0;
+      const int64_t n = lane < P.batch ? ((int64_t)(length + KB - 1) / KB + draft_blocks<KB>(P)) * P.kv_heads : 0;
       int64_t upto = n;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -493,11 +498,12 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmKc, const __grid_constant__
   }
   grid_allow_next();
   Walker walk;
-  walk.begin(P, lane, group);
-  if (warp == 0) {
+  walk.ask(P, lane);            // the lengths are on their way meanwhile
+  if (warp == S::kWarps - 1) {
     tmem_alloc(smem_u32(&tmem_slot), 512);
     tmem_relinquish();
   }
+  walk.begin(P, lane, group);
   tc_fence_before_sync();
   __syncthreads();
   tc_fence_after_sync();
@@ -517,6 +523,11 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmKc, const __grid_constant__
     auto pair_sync = [&]() { asm volatile("bar.sync %0, %1;" ::"r"(1 + s * 4 + quarter), "n"(32 * HALVES) : "memory"); };
     auto stream_sync = [&]() { asm volatile("bar.sync %0, %1;" ::"r"(9 + s), "n"(128 * HALVES) : "memory"); };
     const bool working = s < streams && (SPLIT > 1 || local - lane < here);
+    // Two streams: the two warps of a quarter, which share an exponential unit, take turns at it, so that one's maxima, waits and
+    // transfers fall into the other's exponentials
+    const bool turns = TREE_TURNS && STREAMS == 2 && row0 + kRows + quarter * 32 < rows;
+    auto my_turn = [&]() { asm volatile("bar.sync %0, 64;" ::"r"(1 + s * 4 + quarter) : "memory"); };
+    auto your_turn = [&]() { asm volatile("bar.arrive %0, 64;" ::"r"(1 + (s ^ 1) * 4 + quarter) : "memory"); };
     if (working && SPLIT > 1) {      // the keys that other copies take have weight zero here, always
       float zero[16];
 #pragma unroll
@@ -563,6 +574,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmKc, const __grid_constant__
           else tmem_ld16(tS + (part * HALVES + half) * CW, x[k]);
         }
         tmem_ld_wait();
+        const bool masked = draft || n < CW;
         if (draft) {
 #pragma unroll
           for (int k = 0; k < NCH; ++k) {
@@ -618,12 +630,15 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmKc, const __grid_constant__
           tmem_st_wait();
         }
         const float ref = m_ref == -INFINITY ? 0.f : m_ref;     // -inf - -inf must not be formed
+        if (STREAMS == 2 && turns && (s == 1 || u > 0)) my_turn();
 #pragma unroll
         for (int k = 0; k < NCH; ++k) {
-          l += exp_row<CH>(x[k], scale2, ref);
-          if constexpr (CH == 32) tmem_st_bf16_row32(tP + (part * HALVES + half) * (CW / 2) + k * 16, x[k]);
-          else tmem_st_bf16_row16(tP + (part * HALVES + half) * (CW / 2), x[k]);
+          uint32_t r[CH / 2];
+          if (masked) l += exp_pack_row<CH, 0>(x[k], scale2, ref, r);       // a masked logit, -inf, gives 0
+          else l += exp_pack_row<CH, TREE_SHARE>(x[k], scale2, ref, r);
+          tmem_st_words(tP + (part * HALVES + half) * (CW / 2) + k * 16, r);
         }
+        if (STREAMS == 2 && turns) your_turn();
         tmem_st_wait();
         tc_fence_before_sync();
         mbar_arrive(smem_u32(&bars.p_full[s][buf]));
@@ -756,6 +771,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmKc, const __grid_constant__
         stream_sync();        // the rows have been read: Q of the next unit may take their place
       }
     }
+    if (STREAMS == 2 && turns && working && s == 0 && u > 0) my_turn();     // the last one that was given
   } else if (warp < SOFT + STREAMS) {
     // ------------------------------------------------------------------ MMA issuer of a stream
     const int s = warp - SOFT;
