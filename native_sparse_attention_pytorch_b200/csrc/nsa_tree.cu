@@ -636,9 +636,9 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmKc, const __grid_constant__
           uint32_t r[CH / 2];
           if (masked) l += exp_pack_row<CH, 0>(x[k], scale2, ref, r);       // a masked logit, -inf, gives 0
           else l += exp_pack_row<CH, TREE_SHARE>(x[k], scale2, ref, r);
+          if (STREAMS == 2 && turns && k == NCH - 1) your_turn();
           tmem_st_words(tP + (part * HALVES + half) * (CW / 2) + k * 16, r);
         }
-        if (STREAMS == 2 && turns) your_turn();
         tmem_st_wait();
         tc_fence_before_sync();
         mbar_arrive(smem_u32(&bars.p_full[s][buf]));
