@@ -559,7 +559,9 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmKc, const __grid_constant__
         fence_proxy_async_smem();
         mbar_arrive(smem_u32(&bars.q_full[s]));
       }
-      float m_ref = -INFINITY, l = 0.f;         // l: of this thread's keys
+      // a lane without a row gives weights of zero: ones, of a query of zeros, would cost the products' power (64 / 8 heads of 128, 32
+      // sequences of 16384, back to back: 274 -> 248 us)
+      float m_ref = valid ? -INFINITY : INFINITY, l = 0.f;         // l: of this thread's keys
       for (int j = walk.j0; j < walk.j1; ++j, ++u) {
         const uint32_t buf = u % LOOK, phase = (u / LOOK) & 1;
         const uint32_t tS = tm_lane + buf * kKeys, tP = tm_lane + tP0 + buf * tPstep;

@@ -13,6 +13,9 @@ import torch.nn.functional as F
 from torch import nn
 from torch.autograd import Function
 
+from .rotary import _rotate
+
+FP32_EPS = torch.finfo(torch.float32).eps
 MAX_PIECES = 256          # sixteen-byte pieces per row the kernel keeps in registers
 
 
@@ -96,6 +99,5 @@ def norm_rotate_heads(q, k, q_weight, k_weight, rotary, positions=None, offset=0
     weights [d], or one row per head, [heads, d], both of one form, in the tensors' type or float32.  eps defaults to the
     machine epsilon of fp32.  The norm is not rounded before the rotation.  Differentiable in q, k and the weights (sums
     in a fixed order: the same call gives the same gradients); other arguments as `rotate_heads`."""
-    from .rotary import _rotate
     return _rotate(q, k, q_weight, k_weight, rotary, positions, offset, True,
-                   torch.finfo(torch.float32).eps if eps is None else float(eps), out)
+                   FP32_EPS if eps is None else float(eps), out)

@@ -710,7 +710,6 @@ def decode_step(q, qr, keys, vals, ck, cv, mem_k, mem_v, gates, *, stride, block
 # drafted tokens against a cache
 # --------------------------------------------------------------------------
 
-@torch.no_grad()
 def tree_attend(q, k_cache, v_cache, lengths, k, v, mask=None, *, scale=None, return_lse=False, impl='auto'):
     """Attention of drafted tokens over a cache and over one another, for verifying a tree of them in one step (or, with one
     token, for plain decoding against a dense cache; or, without a mask, for a chunk of a prompt).
@@ -722,12 +721,15 @@ def tree_attend(q, k_cache, v_cache, lengths, k, v, mask=None, *, scale=None, re
     length, or in a drafted row that a token does not see, leaves no trace in it, NaN included.  scale defaults to
     d^-0.5.  No gradient.  Returns out [b, q_heads, t, d], with `return_lse` also its log sum of exponentials (fp32
     [b, q_heads, t]), by which it can be merged with attention over other keys.  See nsa_tree_attend in include/nsa_b200.h."""
-    length = k_cache.shape[2] if lengths is None else 0
-    if isinstance(lengths, int):
+    length = 0
+    if lengths is None:
+        length = k_cache.shape[2]
+    elif isinstance(lengths, int):
         lengths, length = None, lengths
         if not 0 <= length <= k_cache.shape[2]:
             raise L.NsaError(f'length must be between 0 and the capacity {k_cache.shape[2]}, got {length}')
-    L.require_cuda(q, k_cache, v_cache, lengths, k, v, mask)
+    if not q.is_cuda:
+        L.require_cuda(q)
     out, lse = L.host().tree_attend(q, k_cache, v_cache, lengths, length, k, v, mask, q.shape[-1] ** -0.5 if scale is None else scale,
                                     return_lse, L.IMPL_BY_NAME[impl], _status_word(q.device))
     return (out, lse) if return_lse else out

@@ -11,6 +11,8 @@ import torch
 from torch import nn
 from torch.autograd import Function, forward_ad
 
+from . import _lib as L
+
 
 _INV_FREQ = {}
 
@@ -52,7 +54,6 @@ class _Rotate(Function):
 
 
 def _launch(x, cos, sin, inverse, order=None):
-    from . import _lib as L
     from .ops import empty_in_order
     lib = L.load()
     v = 16 // x.element_size()
@@ -159,25 +160,22 @@ class RotaryFrequencies:
         t = self._on.get(device)
         if t is None:
             if torch.cuda.is_current_stream_capturing():
-                from ._lib import NsaError
-                raise NsaError('the frequencies are not on this device yet: call once before a CUDA graph is recorded')
+                raise L.NsaError('the frequencies are not on this device yet: call once before a CUDA graph is recorded')
             t = self._on[device] = self._steps.to(device)
             torch.cuda.current_stream(device).synchronize()     # other streams may read it from now on
         return t
 
 
 def _rotate(q, k, q_weight, k_weight, rotary, positions, offset, norm, eps, out):
-    from . import _lib as L
-    for t in (q, k, q_weight, k_weight, positions):
-        L.require_cuda(t)
     if forward_ad._current_level >= 0:
         raise L.NsaError('the rotation of heads has no forward-mode derivative')
+    if not q.is_cuda:
+        L.require_cuda(q)
     if q.shape[-1] != rotary.dim_head:
         raise L.NsaError(f'the frequencies are for heads of {rotary.dim_head}, not {q.shape[-1]}')
     out_q, out_k = (None, None) if out is None else out
-    y, z = L.host().rotate_heads(q, k, q_weight, k_weight, rotary.steps(q.device), rotary.rotary_dim, rotary.layout == 'half',
-                                 rotary.magnitude, positions, offset, norm, eps, out_q, out_k)
-    return y, z
+    return tuple(L.host().rotate_heads(q, k, q_weight, k_weight, rotary.steps(q.device), rotary.rotary_dim,
+                                       rotary.layout == 'half', rotary.magnitude, positions, offset, norm, eps, out_q, out_k))
 
 
 def rotate_heads(q, k, rotary, positions=None, offset=0, out=None):
