@@ -101,6 +101,50 @@ __device__ __forceinline__ bool sees(const TreeParams& P, int b, int t, int u) {
   return P.mask != nullptr ? P.mask[b * P.m_sb + t * P.m_st + u] != 0 : u <= t;
 }
 
+// Which of N drafted rows from `first` on token t sees, and which of N rows (token, head) from `first` on see drafted row u: bits.  The
+// loads do not depend on one another, so that they are under way all at once.
+template <int N>
+__device__ __forceinline__ uint32_t seen_from(const TreeParams& P, int b, int t, int first) {
+  uint32_t bits = 0;
+  if (P.mask == nullptr) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) bits |= (first + i <= t && first + i < P.tokens ? 1u : 0u) << i;
+    return bits;
+  }
+  const uint8_t* m = P.mask + b * P.m_sb + t * P.m_st;
+  uint8_t v[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) v[i] = m[min(first + i, P.tokens - 1)];
+#pragma unroll
+  for (int i = 0; i < N; ++i) bits |= (v[i] != 0 && first + i < P.tokens ? 1u : 0u) << i;
+  return bits;
+}
+template <int N>
+__device__ __forceinline__ uint32_t seen_by(const TreeParams& P, int b, int first, int u) {
+  uint32_t bits = 0;
+  if (u >= P.tokens) return 0;
+  int t[N], g = first % P.G;
+  t[0] = first / P.G;
+#pragma unroll
+  for (int i = 1; i < N; ++i) {
+    const bool next = ++g == P.G;
+    t[i] = t[i - 1] + next;
+    if (next) g = 0;
+  }
+  if (P.mask == nullptr) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) bits |= (u <= t[i] && t[i] < P.tokens ? 1u : 0u) << i;
+    return bits;
+  }
+  const uint8_t* m = P.mask + b * P.m_sb + u;
+  uint8_t v[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) v[i] = m[min(t[i], P.tokens - 1) * P.m_st];
+#pragma unroll
+  for (int i = 0; i < N; ++i) bits |= (v[i] != 0 && t[i] < P.tokens ? 1u : 0u) << i;
+  return bits;
+}
+
 template <typename T>
 __device__ __forceinline__ const T* row_of(const RowView& r, int b, int h, int64_t n) {
   return (const T*)r.p + b * r.sb + h * r.sh + n * r.sn;
@@ -347,9 +391,6 @@ __global__ void __launch_bounds__(tree_simt::kThreads, 2) tree_simt_kernel(const
 //                   weights would be); the sum adds the exponentials as they are.
 // The accumulator O stays in tensor memory.  It is rescaled lazily: a row keeps its reference maximum until a block exceeds it by
 // more than 2^8.
-// SPLIT.  A tensor-core tile has 128 rows however few there are.  Up to 32 rows are written four times over, and warp w takes keys
-// 32 w .. 32 w + 31 of every block for its copy (its P has zeros elsewhere): a quarter of the exponentials a thread, at no cost in
-// products.  Up to 64 rows twice, for halves.  The copies' results are joined in shared memory (in Q's place) where a unit ends.
 // STREAMS.  Above 128 rows two tiles share the K and V blocks; the softmax of one runs under the products of the other.  Blocks of 64
 // keys, so that tensor memory holds two S buffers of either beside both O: with blocks of 128 and one buffer, S of the next block
 // waited for the products of this one, which waited for its softmax (3800 cycles a block and pair of tiles, 2050 of them products).
@@ -440,7 +481,91 @@ struct Walk {
 // Which of a cache's axes the coordinates move along (an axis of stride zero is one entry in its tensor map)
 struct TreeAxes { int kc_b, kc_h, vc_b, vc_h, k_b, k_h, v_b, v_h; };
 
-template <int D, int STREAMS, int SPLIT>
+// The role of the TMA warp: K and V blocks of all units into the ring, as far ahead as it holds
+template <int D, int KK, int SLOTS>
+__device__ __forceinline__ void fetch_blocks(const TreeParams& P, const TreeAxes& A, const CUtensorMap& tmKc, const CUtensorMap& tmVc, const CUtensorMap& tmK,
+                                             const CUtensorMap& tmV, tree::Walk<KK>& walk, uint32_t ring, tree_tc::Bars& bars, int lane, volatile int* abort_flag) {
+  using namespace ptx;
+  constexpr int NC = D / 64;
+  constexpr uint32_t kSub = KK * 128, kTile = NC * kSub;
+  uint32_t i = 0;
+  for (; walk.unit(P); walk.next(P)) {
+    for (int j = walk.j0; j < walk.j1; ++j) {
+      const bool draft = j >= walk.cached;
+      const int first = (draft ? j - walk.cached : j) * KK;
+#pragma unroll
+      for (int v = 0; v < 2; ++v, ++i) {
+        const uint32_t slot = i % SLOTS, round = i / SLOTS;
+        if (round >= 1) mbar_wait_bounded(smem_u32(&bars.free[slot]), (round - 1) & 1, abort_flag);
+        if (lane == 0) {
+          const CUtensorMap* map = draft ? (v ? &tmV : &tmK) : (v ? &tmVc : &tmKc);
+          const int bb = walk.b * (draft ? (v ? A.v_b : A.k_b) : (v ? A.vc_b : A.kc_b));
+          const int hh = walk.h * (draft ? (v ? A.v_h : A.k_h) : (v ? A.vc_h : A.kc_h));
+          mbar_arrive_expect_tx(smem_u32(&bars.full[slot]), kTile);
+#pragma unroll
+          for (int c = 0; c < NC; ++c) tma_load_4d(ring + slot * kTile + c * kSub, map, smem_u32(&bars.full[slot]), c * 64, first, hh, bb);
+        }
+        __syncwarp();
+      }
+    }
+  }
+  // every request must have landed before the block may exit (also when it gave up)
+  for (uint32_t back = 1; back <= (uint32_t)SLOTS && back <= i; ++back)
+    mbar_wait_drain(smem_u32(&bars.full[(i - back) % SLOTS]), ((i - back) / SLOTS) & 1);
+}
+
+// The role of the mending warp: rows of a V block behind the sequence are cleared, as are drafted values that are not finite
+template <int D, int KK, int SLOTS>
+__device__ __forceinline__ void mend_blocks(const TreeParams& P, tree::Walk<KK>& walk, uint32_t ring, tree_tc::Bars& bars, volatile int* odd_values, int lane,
+                                            volatile int* abort_flag) {
+  using namespace ptx;
+  using tree_tc::kAhead;
+  constexpr int NC = D / 64;
+  constexpr uint32_t kSub = KK * 128, kTile = NC * kSub;
+  uint32_t u = 0;
+  for (int seq = 0; walk.unit(P); walk.next(P), ++seq) {
+    int odd = 0;
+    for (int j = walk.j0; j < walk.j1; ++j, ++u) {
+      const uint32_t slot = (2 * u + 1) % SLOTS, round = (2 * u + 1) / SLOTS;
+      const uint32_t at = ring + slot * kTile;
+      // the K block as well: a slot that holds K and V in turn must not be asked about a phase before the one before it is over
+      mbar_wait_warp(smem_u32(&bars.full[2 * u % SLOTS]), (2 * u / SLOTS) & 1, abort_flag);
+      mbar_wait_warp(smem_u32(&bars.full[slot]), round & 1, abort_flag);
+      const bool draft = j >= walk.cached;
+      const int n = min(KK, (draft ? P.tokens - (j - walk.cached) * KK : walk.length - j * KK));
+      if (draft || n < KK) {
+        if (!draft)       // behind the drafted rows the tile is zero as loaded
+          for (int e = lane; e < (KK - n) * 8 * NC; e += 32)
+            sts_v4(at + (e & (NC - 1)) * kSub + sw128_offset(n + (e / NC) / 8, (e / NC) & 7), make_uint4(0, 0, 0, 0));
+        else
+          for (int e = lane; e < n * 8 * NC; e += 32) {
+            const uint32_t p = at + (e & (NC - 1)) * kSub + sw128_offset((e / NC) / 8, (e / NC) & 7);
+            const uint4 v = lds_v4(p);
+            uint32_t w[4] = {v.x, v.y, v.z, v.w};
+            bool bad = false;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              if ((w[k] & 0x7f80u) == 0x7f80u) { w[k] &= 0xffff0000u; bad = true; }
+              if ((w[k] & 0x7f800000u) == 0x7f800000u) { w[k] &= 0xffffu; bad = true; }
+            }
+            if (bad) {
+              sts_v4(p, make_uint4(w[0], w[1], w[2], w[3]));
+              odd = 1;
+            }
+          }
+        fence_proxy_async_smem();
+        odd = __any_sync(kFullMask, odd);
+      }
+      if (lane == 0) {
+        if (j == walk.j1 - 1) odd_values[seq & 15] = odd;
+        mbar_arrive(smem_u32(&bars.ready[u % kAhead]));
+      }
+      __syncwarp();
+    }
+  }
+}
+
+template <int D, int STREAMS>
 __global__ void __launch_bounds__(tree_tc::Shape<D, STREAMS>::kThreads, 1)
 tree_tc_kernel(const __grid_constant__ CUtensorMap tmKc, const __grid_constant__ CUtensorMap tmVc, const __grid_constant__ CUtensorMap tmK,
                const __grid_constant__ CUtensorMap tmV, const TreeParams P, const TreeAxes A, const int q_vec) {
@@ -451,13 +576,11 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmKc, const __grid_constant__
   constexpr int kKeys = S::KK, LOOK = 2;                // keys of a block; S is computed two blocks ahead of P V
   using Walker = Walk<kKeys>;
   typedef __nv_bfloat16 T;
-  constexpr int NC = S::NC, kSlots = S::kSlots, HALVES = S::kHalves, SOFT = 4 * HALVES * STREAMS;
-  constexpr int RT = STREAMS * kRows / SPLIT;           // rows of the CTA's tile
-  constexpr int CW = kKeys / SPLIT / HALVES;                 // keys of a thread in a block
-  constexpr int CH = CW < 32 ? CW : 32, NCH = CW / CH;  // in pieces
+  constexpr int kSlots = S::kSlots, HALVES = S::kHalves, SOFT = 4 * HALVES * STREAMS;
+  constexpr int RT = STREAMS * kRows;                   // rows of the CTA's tile
+  constexpr int CW = kKeys / HALVES, CH = 32, NCH = CW / CH;      // keys of a thread in a block, in pieces
   constexpr uint32_t kTile = S::kTile, kTileQ = S::kTileQ, kSub = S::kSub;
-  // tensor memory of a stream: two S buffers, O behind them; P over the S it came from, or (copies) in a place of its own
-  constexpr uint32_t tO = 2 * kKeys, tP0 = STREAMS == 1 ? 384 : 0, tPstep = STREAMS == 1 ? 64 : kKeys;
+  constexpr uint32_t tO = 2 * kKeys;                    // tensor memory of a stream: two S buffers (P over the S it came from), O behind them
   extern __shared__ __align__(1024) uint8_t tree_tc_smem[];
   __shared__ int abort_flag;
   __shared__ uint32_t tmem_slot;
@@ -472,7 +595,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmKc, const __grid_constant__
   const int rows = P.tokens * P.G, row0 = tile * RT, here = min(RT, rows - row0);     // this tile's rows
   const int streams = STREAMS == 2 && here > kRows ? 2 : 1;
   // quarters of the tensor-core tile with rows, of a stream
-  auto active = [&](int s) { return SPLIT > 1 ? 4 : max(0, min(4, (here - s * kRows + 31) / 32)); };
+  auto active = [&](int s) { return max(0, min(4, (here - s * kRows + 31) / 32)); };
 
   if (tid == 0) {
     abort_flag = sQ0 & 1023u ? 1 : 0;                   // the tiles would be mis-swizzled: report instead of computing
@@ -512,30 +635,19 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmKc, const __grid_constant__
   if (warp < SOFT) {
     // ------------------------------------------------------------------ softmax
     const int s = warp / (4 * HALVES), quarter = warp & 3, half = HALVES > 1 ? (warp >> 2) & 1 : 0;
-    const int part = quarter * SPLIT / 4;                                     // which keys of a block
     const int lane_row = quarter * 32 + lane;                                 // row of the tensor-core tile
-    const int local = s * kRows + (SPLIT == 1 ? lane_row : lane_row % RT);    // row of the CTA's tile
+    const int local = s * kRows + lane_row;                                   // row of the CTA's tile
     const int row = row0 + local, t = row / P.G, g = row - t * P.G;
     const bool valid = local < here;
     const uint32_t tm_lane = tm + s * 256 + ((uint32_t)(quarter * 32) << 16);
     const float scale2 = P.scale * kLog2e;
-    uint8_t* const region = tree_tc_smem + s * kTileQ;
     auto pair_sync = [&]() { asm volatile("bar.sync %0, %1;" ::"r"(1 + s * 4 + quarter), "n"(32 * HALVES) : "memory"); };
-    auto stream_sync = [&]() { asm volatile("bar.sync %0, %1;" ::"r"(9 + s), "n"(128 * HALVES) : "memory"); };
-    const bool working = s < streams && (SPLIT > 1 || local - lane < here);
+    const bool working = s < streams && local - lane < here;
     // Two streams: the two warps of a quarter, which share an exponential unit, take turns at it, so that one's maxima, waits and
     // transfers fall into the other's exponentials
     const bool turns = TREE_TURNS && STREAMS == 2 && row0 + kRows + quarter * 32 < rows;
     auto my_turn = [&]() { asm volatile("bar.sync %0, 64;" ::"r"(1 + s * 4 + quarter) : "memory"); };
     auto your_turn = [&]() { asm volatile("bar.arrive %0, 64;" ::"r"(1 + (s ^ 1) * 4 + quarter) : "memory"); };
-    if (working && SPLIT > 1) {      // the keys that other copies take have weight zero here, always
-      float zero[16];
-#pragma unroll
-      for (int i = 0; i < 16; ++i) zero[i] = 0.f;
-#pragma unroll 1
-      for (int c = half * (128 / HALVES); c < (half + 1) * (128 / HALVES); c += 16) tmem_st16(tm_lane + tP0 + c, zero);
-      tmem_st_wait();
-    }
     uint32_t u = 0;
     for (int seq = 0; working && walk.unit(P); walk.next(P), ++seq) {
       // the query's row, swizzled as the products want it
@@ -564,16 +676,15 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmKc, const __grid_constant__
       float m_ref = valid ? -INFINITY : INFINITY, l = 0.f;         // l: of this thread's keys
       for (int j = walk.j0; j < walk.j1; ++j, ++u) {
         const uint32_t buf = u % LOOK, phase = (u / LOOK) & 1;
-        const uint32_t tS = tm_lane + buf * kKeys, tP = tm_lane + tP0 + buf * tPstep;
+        const uint32_t tS = tm_lane + buf * kKeys, tP = tS;
         const bool draft = j >= walk.cached;
-        const int first = (draft ? j - walk.cached : j) * kKeys + (part * HALVES + half) * CW, n = (draft ? P.tokens : walk.length) - first;
+        const int first = (draft ? j - walk.cached : j) * kKeys + half * CW, n = (draft ? P.tokens : walk.length) - first;
         float x[NCH][CH];
         mbar_wait_warp(smem_u32(&bars.s_full[s][buf]), phase, &abort_flag);
         tc_fence_after_sync();
 #pragma unroll
         for (int k = 0; k < NCH; ++k) {
-          if constexpr (CH == 32) tmem_ld32(tS + (part * HALVES + half) * CW + k * 32, x[k]);
-          else tmem_ld16(tS + (part * HALVES + half) * CW, x[k]);
+          tmem_ld32(tS + half * CW + k * 32, x[k]);
         }
         tmem_ld_wait();
         const bool masked = draft || n < CW;
@@ -581,11 +692,8 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmKc, const __grid_constant__
 #pragma unroll
           for (int k = 0; k < NCH; ++k) {
             uint32_t seen = 0;
-            if (valid) {
-#pragma unroll 8
-              for (int i = 0; i < CH; ++i)
-                if (k * CH + i < n && sees(P, walk.b, t, first + k * CH + i)) seen |= 1u << i;
-            }
+#pragma unroll 1
+            for (int i = 0; valid && i < CH; i += 8) seen |= seen_from<8>(P, walk.b, t, first + k * CH + i) << i;
 #pragma unroll
             for (int i = 0; i < CH; ++i)
               if (!(seen >> i & 1)) x[k][i] = -INFINITY;
@@ -639,7 +747,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmKc, const __grid_constant__
           if (masked) l += exp_pack_row<CH, 0>(x[k], scale2, ref, r);       // a masked logit, -inf, gives 0
           else l += exp_pack_row<CH, TREE_SHARE>(x[k], scale2, ref, r);
           if (STREAMS == 2 && turns && k == NCH - 1) your_turn();
-          tmem_st_words(tP + (part * HALVES + half) * (CW / 2) + k * 16, r);
+          tmem_st_words(tP + half * (CW / 2) + k * 16, r);
         }
         tmem_st_wait();
         tc_fence_before_sync();
@@ -692,86 +800,18 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmKc, const __grid_constant__
         else if (P.lse != nullptr)
           P.lse[((int64_t)walk.b * P.q_heads + head) * P.tokens + token] = l_row == 0.f ? -INFINITY : (m_row + log2f(l_row)) * kLn2;
       };
-      if constexpr (SPLIT == 1) {
 #pragma unroll 1
-        for (int c = half * (D / HALVES); c < (half + 1) * (D / HALVES); c += 32) {
-          float o[32];
-          tmem_ld32(tm_lane + tO + c, o);
-          tmem_ld_wait();
-          if (valid)
+      for (int c = half * (D / HALVES); c < (half + 1) * (D / HALVES); c += 32) {
+        float o[32];
+        tmem_ld32(tm_lane + tO + c, o);
+        tmem_ld_wait();
+        if (valid)
 #pragma unroll
-            for (int k = 0; k < 4; ++k) store8(local, t, walk.h * P.G + g, c + 8 * k, l, o + 8 * k);
-          __syncwarp();
-        }
-        if (valid && half == 0) store_stats(local, t, walk.h * P.G + g, m_ref, l);
-        if (HALVES > 1) pair_sync();        // both have read the sums: the next unit's first block may write the same place
-      } else {
-        // join the copies: the upper half of them leaves its rows in Q's place, the lower half adds its own, then all threads
-        // take rows apart
-        float2* const joined = reinterpret_cast<float2*>(&xchg[s][(u + 1) % LOOK][0][0]);    // maximum and sum of every copy of a row
-        if (half == 0) joined[lane_row] = make_float2(m_ref, l);
-        stream_sync();
-        float top = -INFINITY, sum = 0.f;
-#pragma unroll
-        for (int k = 0; k < SPLIT; ++k) top = fmaxf(top, joined[k * RT + local].x);
-        const float base = top == -INFINITY ? 0.f : top;
-#pragma unroll
-        for (int k = 0; k < SPLIT; ++k) sum += joined[k * RT + local].y * ex2(joined[k * RT + local].x - base);
-        const float w = ex2(m_ref - base);
-        // row `local` of place k, 16-byte pieces exchanged against bank conflicts
-        auto piece = [&](int k, int r, int c4) { return reinterpret_cast<float4*>(region + (size_t)(k * RT + r) * (D * 4)) + (c4 ^ (r & 7)); };
-        if (part >= SPLIT / 2) {
-#pragma unroll 1
-          for (int c = half * (D / HALVES); c < (half + 1) * (D / HALVES); c += 16) {
-            float o[16];
-            tmem_ld16(tm_lane + tO + c, o);
-            tmem_ld_wait();
-#pragma unroll
-            for (int k = 0; k < 4; ++k)
-              if (valid) *piece(part - SPLIT / 2, local, c / 4 + k) = make_float4(o[4 * k] * w, o[4 * k + 1] * w, o[4 * k + 2] * w, o[4 * k + 3] * w);
-          }
-        }
-        stream_sync();
-        if (part < SPLIT / 2) {
-#pragma unroll 1
-          for (int c = half * (D / HALVES); c < (half + 1) * (D / HALVES); c += 16) {
-            float o[16];
-            tmem_ld16(tm_lane + tO + c, o);
-            tmem_ld_wait();
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              if (!valid) continue;
-              float4* at = piece(part, local, c / 4 + k);
-              const float4 v = *at;
-              *at = make_float4(v.x + o[4 * k] * w, v.y + o[4 * k + 1] * w, v.z + o[4 * k + 2] * w, v.w + o[4 * k + 3] * w);
-            }
-          }
-        }
-        if (half == 0 && (quarter == 0 || (SPLIT == 2 && quarter == 1))) {
-          if (valid) store_stats(local, t, walk.h * P.G + g, top, sum);
-        }
-        stream_sync();
-        for (int e = half * 128 + lane_row; e < here * (D / 8); e += 128 * HALVES) {
-          const int r = e / (D / 8), c = (e - r * (D / 8)) * 8, rr = row0 + r, token = rr / P.G;
-          float o[8], total = 0.f, high = -INFINITY;
-#pragma unroll
-          for (int k = 0; k < SPLIT; ++k) high = fmaxf(high, joined[k * RT + r].x);
-          const float low = high == -INFINITY ? 0.f : high;
-#pragma unroll
-          for (int k = 0; k < SPLIT; ++k) total += joined[k * RT + r].y * ex2(joined[k * RT + r].x - low);
-#pragma unroll
-          for (int k = 0; k < 2; ++k) {
-            float4 v = *piece(0, r, c / 4 + k);
-            if constexpr (SPLIT == 4) {
-              const float4 z = *piece(1, r, c / 4 + k);
-              v.x += z.x; v.y += z.y; v.z += z.z; v.w += z.w;
-            }
-            o[4 * k] = v.x; o[4 * k + 1] = v.y; o[4 * k + 2] = v.z; o[4 * k + 3] = v.w;
-          }
-          store8(r, token, walk.h * P.G + rr - token * P.G, c, total, o);
-        }
-        stream_sync();        // the rows have been read: Q of the next unit may take their place
+          for (int k = 0; k < 4; ++k) store8(local, t, walk.h * P.G + g, c + 8 * k, l, o + 8 * k);
+        __syncwarp();
       }
+      if (valid && half == 0) store_stats(local, t, walk.h * P.G + g, m_ref, l);
+      if (HALVES > 1) pair_sync();        // both have read the sums: the next unit's first block may write the same place
     }
     if (STREAMS == 2 && turns && working && s == 0 && u > 0) my_turn();     // the last one that was given
   } else if (warp < SOFT + STREAMS) {
@@ -808,7 +848,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmKc, const __grid_constant__
           __syncwarp();
           tc_fence_after_sync();
           const uint64_t dV = smem_desc_sw128(sRing + slot * kTile, kSub);
-          const uint32_t tP = ts + tP0 + (u % LOOK) * tPstep;
+          const uint32_t tP = ts + (u % LOOK) * kKeys;
 #pragma unroll
           for (int k = 0; k < kKeys / 16; ++k) mma_bf16_tmem_a_elect(ts + tO, tP + k * 8, desc_advance(dV, k * 2048), idO, t > 0 || k > 0);
           mma_commit_elect(smem_u32(&bars.pv_done[s][u % LOOK]));
@@ -821,79 +861,363 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmKc, const __grid_constant__
       mbar_wait_drain(smem_u32(&bars.drain[s]), 0);
     }
   } else if (warp == SOFT + STREAMS) {
-    // ------------------------------------------------------------------ TMA
-    uint32_t i = 0;
-    for (; walk.unit(P); walk.next(P)) {
-      for (int j = walk.j0; j < walk.j1; ++j) {
-        const bool draft = j >= walk.cached;
-        const int first = (draft ? j - walk.cached : j) * kKeys;
-#pragma unroll
-        for (int v = 0; v < 2; ++v, ++i) {
-          const uint32_t slot = i % kSlots, round = i / kSlots;
-          if (round >= 1) mbar_wait_bounded(smem_u32(&bars.free[slot]), (round - 1) & 1, &abort_flag);
-          if (lane == 0) {
-            const CUtensorMap* map = draft ? (v ? &tmV : &tmK) : (v ? &tmVc : &tmKc);
-            const int bb = walk.b * (draft ? (v ? A.v_b : A.k_b) : (v ? A.vc_b : A.kc_b));
-            const int hh = walk.h * (draft ? (v ? A.v_h : A.k_h) : (v ? A.vc_h : A.kc_h));
-            mbar_arrive_expect_tx(smem_u32(&bars.full[slot]), kTile);
-#pragma unroll
-            for (int c = 0; c < NC; ++c) tma_load_4d(sRing + slot * kTile + c * kSub, map, smem_u32(&bars.full[slot]), c * 64, first, hh, bb);
-          }
-          __syncwarp();
-        }
-      }
-    }
-    // every request must have landed before the block may exit (also when it gave up)
-    for (uint32_t back = 1; back <= (uint32_t)kSlots && back <= i; ++back)
-      mbar_wait_drain(smem_u32(&bars.full[(i - back) % kSlots]), ((i - back) / kSlots) & 1);
+    fetch_blocks<D, kKeys, kSlots>(P, A, tmKc, tmVc, tmK, tmV, walk, sRing, bars, lane, &abort_flag);
   } else {
-    // ------------------------------------------------------------------ mending of V blocks
-    uint32_t u = 0;
-    for (int seq = 0; walk.unit(P); walk.next(P), ++seq) {
-      int odd = 0;
-      for (int j = walk.j0; j < walk.j1; ++j, ++u) {
-        const uint32_t slot = (2 * u + 1) % kSlots, round = (2 * u + 1) / kSlots;
-        const uint32_t at = sRing + slot * kTile;
-        // the K block as well: a slot that holds K and V in turn must not be asked about a phase before the one before it is over
-        mbar_wait_warp(smem_u32(&bars.full[2 * u % kSlots]), (2 * u / kSlots) & 1, &abort_flag);
-        mbar_wait_warp(smem_u32(&bars.full[slot]), round & 1, &abort_flag);
-        const bool draft = j >= walk.cached;
-        const int n = min(kKeys, (draft ? P.tokens - (j - walk.cached) * kKeys : walk.length - j * kKeys));
-        if (draft || n < kKeys) {
-          if (!draft)       // behind the drafted rows the tile is zero as loaded
-            for (int e = lane; e < (kKeys - n) * 8 * NC; e += 32)
-              sts_v4(at + (e & (NC - 1)) * kSub + sw128_offset(n + (e / NC) / 8, (e / NC) & 7), make_uint4(0, 0, 0, 0));
-          else
-            for (int e = lane; e < n * 8 * NC; e += 32) {
-              const uint32_t p = at + (e & (NC - 1)) * kSub + sw128_offset((e / NC) / 8, (e / NC) & 7);
-              const uint4 v = lds_v4(p);
-              uint32_t w[4] = {v.x, v.y, v.z, v.w};
-              bool bad = false;
-#pragma unroll
-              for (int k = 0; k < 4; ++k) {
-                if ((w[k] & 0x7f80u) == 0x7f80u) { w[k] &= 0xffff0000u; bad = true; }
-                if ((w[k] & 0x7f800000u) == 0x7f800000u) { w[k] &= 0xffffu; bad = true; }
-              }
-              if (bad) {
-                sts_v4(p, make_uint4(w[0], w[1], w[2], w[3]));
-                odd = 1;
-              }
-            }
-          fence_proxy_async_smem();
-          odd = __any_sync(kFullMask, odd);
-        }
-        if (lane == 0) {
-          if (j == walk.j1 - 1) odd_values[seq & 15] = odd;
-          mbar_arrive(smem_u32(&bars.ready[u % kAhead]));
-        }
-        __syncwarp();
-      }
-    }
+    mend_blocks<D, kKeys, kSlots>(P, walk, sRing, bars, odd_values, lane, &abort_flag);
   }
 
   tc_fence_before_sync();
   __syncthreads();
   if (warp == 0) tmem_dealloc(tm, 512);
+  if (tid == 0 && abort_flag && P.status != nullptr) atomicOr(P.status, 1);
+}
+
+// ---- few rows: keys along the tensor-core tile's rows --------------------------------------------
+
+// Up to 64 rows would leave most of a tile of 128 rows empty.  Here the keys of a block are its rows and the queries its columns (N, a
+// multiple of 16): S^T = K Q^T [128 keys x N], O^T += V^T P^T [dim_head x N].  A thread has a key (two or four threads share one, eight or
+// sixteen columns each) and exponentials for the rows there are; P^T goes through shared memory, K-major as the products want it.
+//   * The reference maxima are one per column, the same for all threads, in shared memory.  While no logit exceeds its column's by
+//     more than 2^8 (one vote of all softmax warps a block) nothing is reduced over the keys; else, and for the first block of a unit
+//     and those of the drafted rows, the maxima are taken, O^T and the sums rescaled.
+//   * Sums stay with the threads, a key each, until a unit ends.
+//   * The transposed accumulator leaves whole rows of the output side by side.
+// Against the tile with rows as rows and copies of them over the keys: XXX
+namespace tree_few {
+constexpr int KK = 128;
+template <int D, int N>
+struct Shape {
+  static constexpr int NC = D / 64, kParts = N == 64 ? 4 : 2;      // threads that share a key
+  static constexpr int kSoftWarps = 4 * kParts, kSoft = 32 * kSoftWarps, kThreads = kSoft + 96;
+  static constexpr uint32_t kTile = NC * KK * 128, kQ = NC * N * 128, kP = N * 256;      // K or V block; queries; P of a block
+  static constexpr int kFit = (int)((14 * 16384 - kQ - 2 * kP) / kTile), kSlots = kFit < tree_tc::kMostSlots ? kFit : tree_tc::kMostSlots;
+  static constexpr uint32_t kBytes = kSlots * kTile + kQ + 2 * kP;
+};
+}  // namespace tree_few
+
+namespace tree_few {
+// Over the lanes of a warp, the maximum (or the sum) of each of NT columns; lane c has that of column c (modulo NT).  Every step
+// gives half of the columns away: 31 exchanges for 32 columns.
+template <int NT, bool MAX>
+__device__ __forceinline__ float reduce_columns(float (&v)[NT]) {
+  const int lane = threadIdx.x & 31;
+  auto join = [](float a, float b) { return MAX ? fmaxf(a, b) : a + b; };
+#pragma unroll
+  for (int o = NT / 2; o > 0; o >>= 1) {
+    const bool upper = lane & o;
+#pragma unroll
+    for (int i = 0; i < o; ++i) {
+      const float keep = upper ? v[i + o] : v[i], give = upper ? v[i] : v[i + o];
+      v[i] = join(keep, __shfl_xor_sync(kFullMask, give, o));
+    }
+  }
+#pragma unroll
+  for (int o = NT; o < 32; o <<= 1) v[0] = join(v[0], __shfl_xor_sync(kFullMask, v[0], o));
+  return v[0];
+}
+}  // namespace tree_few
+
+template <int D, int N>
+__global__ void __launch_bounds__(tree_few::Shape<D, N>::kThreads, 1)
+tree_few_kernel(const __grid_constant__ CUtensorMap tmKc, const __grid_constant__ CUtensorMap tmVc, const __grid_constant__ CUtensorMap tmK,
+                const __grid_constant__ CUtensorMap tmV, const TreeParams P, const TreeAxes A, const int q_vec) {
+  using namespace ptx;
+  using namespace tree;
+  using tree_tc::Bars;
+  using tree_tc::kAhead;
+  using namespace tree_few;
+  using S = Shape<D, N>;
+  typedef __nv_bfloat16 T;
+  constexpr int kSlots = S::kSlots, kSoftWarps = S::kSoftWarps, kSoft = S::kSoft, NT = N / S::kParts;      // NT: columns of a thread
+  constexpr uint32_t kSub = KK * 128, kTile = S::kTile, tO = 2 * N;    // tensor memory: two S^T buffers, O^T
+  extern __shared__ __align__(1024) uint8_t tree_few_smem[];
+  __shared__ int abort_flag;
+  __shared__ uint32_t tmem_slot;
+  __shared__ __align__(8) Bars bars;
+  __shared__ volatile int odd_values[16];               // by unit: a drafted value is not finite
+  // by column: the reference maximum (base 2; -inf: nothing seen yet), what is added to the logits (0 for that; -inf for a column
+  // without a row, whose weights are then zero), the factor of a rescaling, at a unit's end the sum
+  __shared__ __align__(16) float ref[N], off[N], factor[N], sums[N];
+  __shared__ float found[4][N];                         // maxima, and sums at a unit's end, of the quarters of the keys
+
+  const uint32_t sRing = smem_u32(tree_few_smem), sQ = sRing + kSlots * kTile, sP = sQ + S::kQ;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int group = blockIdx.x, here = P.tokens * P.G;   // one tile holds all rows
+
+  if (tid == 0) {
+    abort_flag = sRing & 1023u ? 1 : 0;                  // the tiles would be mis-swizzled: report instead of computing
+    for (int i = 0; i < kSlots; ++i) {
+      mbar_init(smem_u32(&bars.full[i]), 1);
+      mbar_init(smem_u32(&bars.free[i]), 1);
+    }
+    for (int i = 0; i < kAhead; ++i) mbar_init(smem_u32(&bars.ready[i]), 1);
+    mbar_init(smem_u32(&bars.q_full[0]), kSoft);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(smem_u32(&bars.s_full[0][i]), 1);
+      mbar_init(smem_u32(&bars.p_full[0][i]), kSoft);
+      mbar_init(smem_u32(&bars.pv_done[0][i]), 1);
+    }
+    mbar_init(smem_u32(&bars.drain[0]), 1);
+    fence_mbar_init();
+    prefetch_tensormap(&tmKc);
+    prefetch_tensormap(&tmVc);
+    prefetch_tensormap(&tmK);
+    prefetch_tensormap(&tmV);
+  }
+  grid_allow_next();
+  Walk<KK> walk;
+  walk.ask(P, lane);            // the lengths are on their way meanwhile
+  if (warp == kSoftWarps) {
+    tmem_alloc(smem_u32(&tmem_slot), 256);
+    tmem_relinquish();
+  }
+  walk.begin(P, lane, group);
+  tc_fence_before_sync();
+  __syncthreads();
+  tc_fence_after_sync();
+  const uint32_t tm = tmem_slot;
+
+  if (warp < kSoftWarps) {
+    // ------------------------------------------------------------------ softmax
+    const int quarter = warp & 3, key = quarter * 32 + lane, col0 = (warp >> 2) * NT;
+    const uint32_t tm_lane = tm + ((uint32_t)(quarter * 32) << 16);
+    const float scale2 = P.scale * kLog2e;
+    const uint64_t scale = pack2(scale2, scale2);
+    auto soft_sync = [&]() { asm volatile("bar.sync 1, %0;" ::"n"(kSoft) : "memory"); };
+    auto soft_any = [&](bool mine) {
+      uint32_t any;
+      asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbar.red.or.pred q, 1, %2, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+                   : "=r"(any) : "r"((uint32_t)mine), "n"(kSoft) : "memory");
+      return any != 0;
+    };
+    // where this key's weight of column c lies in a P tile: rows of 64 keys, 16-byte pieces exchanged by row & 7
+    uint32_t place[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) place[k] = sP + (quarter >> 1) * (N * 128) + ((((key & 63) >> 3) ^ k) << 4) + (key & 7) * 2;
+    uint32_t u = 0;
+    for (int seq = 0; walk.unit(P); walk.next(P), ++seq) {
+      {
+        constexpr int kPieces = (N * (D / 8) + kSoft - 1) / kSoft;
+        uint4 v[kPieces];
+#pragma unroll
+        for (int i = 0; i < kPieces; ++i) {
+          const int e = tid + i * kSoft, r = e / (D / 8), c = e % (D / 8), t = r / P.G, g = r - t * P.G;
+          v[i] = make_uint4(0, 0, 0, 0);
+          if (r < here && c * 8 < P.d) {
+            const T* src = row_of<T>(P.q, walk.b, walk.h * P.G + g, t) + c * 8;
+            if (q_vec) v[i] = *reinterpret_cast<const uint4*>(src);
+            else {
+              __align__(16) T x[8];
+#pragma unroll
+              for (int k = 0; k < 8; ++k) x[k] = src[k];
+              v[i] = *reinterpret_cast<const uint4*>(x);
+            }
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < kPieces; ++i) {
+          const int e = tid + i * kSoft, r = e / (D / 8), c = e % (D / 8);
+          if (r < N) sts_v4(sQ + (c / 8) * (N * 128) + sw128_offset(r, c & 7), v[i]);
+        }
+      }
+      fence_proxy_async_smem();
+      mbar_arrive(smem_u32(&bars.q_full[0]));
+      if (tid < N) {
+        ref[tid] = -INFINITY;
+        off[tid] = tid < here ? 0.f : -INFINITY;
+      }
+      float l[NT];
+#pragma unroll
+      for (int c = 0; c < NT; ++c) l[c] = 0.f;
+      for (int j = walk.j0; j < walk.j1; ++j, ++u) {
+        const uint32_t buf = u & 1, phase = (u >> 1) & 1;
+        const bool draft = j >= walk.cached;
+        const int at = (draft ? j - walk.cached : j) * KK + key;       // row of the cache, or drafted row
+        float x[NT];
+        mbar_wait_warp(smem_u32(&bars.s_full[0][buf]), phase, &abort_flag);
+        tc_fence_after_sync();
+        if constexpr (NT == 8) tmem_ld8(tm_lane + buf * N + col0, x);
+        else tmem_ld16(tm_lane + buf * N + col0, x);
+        tmem_ld_wait();
+        if (draft) {
+          const uint32_t seen = seen_by<NT>(P, walk.b, col0, at);
+#pragma unroll
+          for (int c = 0; c < NT; ++c)
+            if (!(seen >> c & 1)) x[c] = -INFINITY;
+        } else if (at >= walk.length) {
+#pragma unroll
+          for (int c = 0; c < NT; ++c) x[c] = -INFINITY;
+        }
+        float y[NT];
+        auto shift = [&]() {
+#pragma unroll
+          for (int c = 0; c < NT; c += 4) {
+            const float4 o = *reinterpret_cast<const float4*>(off + col0 + c);
+            unpack2(fma2(pack2(x[c], x[c + 1]), scale, pack2(o.x, o.y)), y[c], y[c + 1]);
+            unpack2(fma2(pack2(x[c + 2], x[c + 3]), scale, pack2(o.z, o.w)), y[c + 2], y[c + 3]);
+          }
+        };
+        bool renew = j == walk.j0 || draft;
+        if (!renew) {
+          shift();
+          renew = soft_any(max_row<NT>(y) > 8.f);
+        }
+        if (renew) {
+          // the columns' maxima over the keys; columns that outgrew their reference get a new one
+#pragma unroll
+          for (int c = 0; c < NT; ++c) y[c] = x[c];
+          const float mine = reduce_columns<NT, true>(y);
+          if (lane < NT) found[quarter][col0 + lane] = mine;
+          soft_sync();
+          if (tid < here) {
+            const float m2 = fmaxf(fmaxf(found[0][tid], found[1][tid]), fmaxf(found[2][tid], found[3][tid])) * scale2, old = ref[tid];
+            const bool grown = old == -INFINITY ? m2 > old || m2 != m2 : m2 > old + 8.f;
+            factor[tid] = grown && old != -INFINITY ? ex2(old - m2) : 1.f;
+            if (grown) { ref[tid] = m2; off[tid] = -m2; }
+          } else if (tid < N) {
+            factor[tid] = 1.f;
+          }
+          soft_sync();
+#pragma unroll
+          for (int c = 0; c < NT; ++c) l[c] *= factor[col0 + c];
+          if (j > walk.j0) {
+            mbar_wait_warp(smem_u32(&bars.pv_done[0][(u - 1) & 1]), ((u - 1) >> 1) & 1, &abort_flag);
+            tc_fence_after_sync();
+#pragma unroll
+            for (int c = 0; c < NT; c += 8) {
+              float o[8];
+              tmem_ld8(tm_lane + tO + col0 + c, o);
+              tmem_ld_wait();
+#pragma unroll
+              for (int i = 0; i < 8; ++i) o[i] *= factor[col0 + c + i];
+              tmem_st8(tm_lane + tO + col0 + c, o);
+            }
+            tmem_st_wait();
+          }
+          shift();
+        }
+#pragma unroll
+        for (int c = 0; c < NT; ++c) y[c] = ex2(y[c]);
+#pragma unroll
+        for (int c = 0; c < NT; c += 2) {
+          unpack2(add2(pack2(l[c], l[c + 1]), pack2(y[c], y[c + 1])), l[c], l[c + 1]);
+          const uint32_t w = pack_bf16(y[c], y[c + 1]);
+          sts_u16(place[c & 7] + buf * S::kP + (col0 + c) * 128, (uint16_t)w);
+          sts_u16(place[(c + 1) & 7] + buf * S::kP + (col0 + c + 1) * 128, (uint16_t)(w >> 16));
+        }
+        fence_proxy_async_smem();
+        tc_fence_before_sync();
+        mbar_arrive(smem_u32(&bars.p_full[0][buf]));
+      }
+      // the unit's end: sums over the keys, then O^T of this CTA's blocks, complete or a partial result
+      const float mine = reduce_columns<NT, false>(l);
+      if (lane < NT) found[quarter][col0 + lane] = mine;
+      soft_sync();
+      const bool whole = walk.j0 == 0 && walk.j1 == walk.per_unit;
+      const int64_t slot = (int64_t)blockIdx.x * 2 + (walk.j0 == 0 ? 1 : 0);
+      if (tid < here) {
+        const float sum = (found[0][tid] + found[1][tid]) + (found[2][tid] + found[3][tid]);
+        sums[tid] = sum;
+        const int t = tid / P.G, g = tid - t * P.G;
+        if (!whole) P.stats[slot * N + tid] = make_float2(ref[tid], sum);
+        else if (P.lse != nullptr)
+          P.lse[((int64_t)walk.b * P.q_heads + walk.h * P.G + g) * P.tokens + t] = sum == 0.f ? -INFINITY : (ref[tid] + log2f(sum)) * kLn2;
+      }
+      mbar_wait_warp(smem_u32(&bars.pv_done[0][(u - 1) & 1]), ((u - 1) >> 1) & 1, &abort_flag);
+      tc_fence_after_sync();
+      soft_sync();
+      float o[NT];
+      if constexpr (NT == 8) tmem_ld8(tm_lane + tO + col0, o);
+      else tmem_ld16(tm_lane + tO + col0, o);
+      tmem_ld_wait();
+      // 128 features lie in 128 lanes, 64 in the first half of every quarter
+      const int f = D == 128 ? key : quarter * 16 + lane;
+      if (D == 128 || lane < 16) {
+        const bool odd = odd_values[seq & 15] != 0;
+        const int u0 = max(0, walk.j0 - walk.cached) * KK, u1 = min(P.tokens, (walk.j1 - walk.cached) * KK);
+        if (odd) {           // values that are not finite, of drafted rows that a row sees
+          for (int uu = u0; uu < u1; ++uu) {
+            const float z = f < P.d ? __bfloat162float(row_of<T>(P.v, walk.b, walk.h, uu)[f]) : 0.f;
+            if (isfinite(z)) continue;
+#pragma unroll
+            for (int c = 0; c < NT; ++c)
+              if (col0 + c < here && sees(P, walk.b, (col0 + c) / P.G, uu)) o[c] += z;
+          }
+        }
+        if (!whole) {
+          float* dst = P.partial + (slot * N + col0) * D + f;
+#pragma unroll
+          for (int c = 0; c < NT; ++c)
+            if (col0 + c < here) dst[c * D] = o[c];
+        } else if (f < P.d) {
+          int t = col0 / P.G, g = col0 - t * P.G;
+          T* dst = const_cast<T*>(row_of<T>(P.out, walk.b, walk.h * P.G + g, t)) + f;
+#pragma unroll
+          for (int c = 0; c < NT; ++c) {
+            if (col0 + c < here) {
+              const float sum = sums[col0 + c], inv = sum > 0.f ? 1.f / sum : (sum == 0.f ? 0.f : sum);      // a sum that is NaN stays NaN
+              *dst = __float2bfloat16_rn(o[c] * inv);
+            }
+            dst += P.out.sh;
+            if (++g == P.G) {            // the next token's first head
+              g = 0;
+              dst += P.out.sn - P.G * P.out.sh;
+            }
+          }
+        }
+      }
+      soft_sync();        // sums and maxima have been read: the next unit may write the same places
+    }
+  } else if (warp == kSoftWarps) {
+    // ------------------------------------------------------------------ MMA issuer
+    constexpr uint32_t idS = instr_desc_bf16(128, N, false, false);
+    constexpr uint32_t idO = instr_desc_bf16(D, N, true, false);
+    const uint64_t dQ = smem_desc_sw128(sQ, 16);
+    uint32_t u = 0, su = 0, units = 0;      // blocks whose O, whose S has been issued
+    auto issue_s = [&]() {
+      const uint32_t slot = 2 * su % kSlots, round = 2 * su / kSlots;
+      mbar_wait_bounded(smem_u32(&bars.full[slot]), round & 1, &abort_flag);
+      __syncwarp();
+      tc_fence_after_sync();
+      const uint64_t dK = smem_desc_sw128(sRing + slot * kTile, 16);
+#pragma unroll
+      for (int k = 0; k < D / 16; ++k)
+        mma_bf16_elect(tm + (su & 1) * N, desc_advance(dK, (k / 4) * kSub + (k % 4) * 32), desc_advance(dQ, (k / 4) * (N * 128) + (k % 4) * 32), idS, k > 0);
+      mma_commit_elect(smem_u32(&bars.s_full[0][su & 1]));
+      mma_commit_elect(smem_u32(&bars.free[slot]));
+      ++su;
+    };
+    for (; walk.unit(P); walk.next(P), ++units) {
+      const int nb = walk.j1 - walk.j0;
+      mbar_wait_bounded(smem_u32(&bars.q_full[0]), units & 1, &abort_flag);
+      for (int t = 0; t < 2 && t < nb; ++t) issue_s();
+      for (int t = 0; t < nb; ++t, ++u) {
+        const uint32_t slot = (2 * u + 1) % kSlots;
+        mbar_wait_bounded(smem_u32(&bars.ready[u % kAhead]), (u / kAhead) & 1, &abort_flag);
+        mbar_wait_bounded(smem_u32(&bars.p_full[0][u & 1]), (u >> 1) & 1, &abort_flag);
+        __syncwarp();
+        tc_fence_after_sync();
+        const uint64_t dV = smem_desc_sw128(sRing + slot * kTile, kSub), dP = smem_desc_sw128(sP + (u & 1) * S::kP, 16);
+#pragma unroll
+        for (int k = 0; k < KK / 16; ++k)
+          mma_bf16_elect(tm + tO, desc_advance(dV, k * 2048), desc_advance(dP, (k / 4) * (N * 128) + (k % 4) * 32), idO, t > 0 || k > 0);
+        mma_commit_elect(smem_u32(&bars.pv_done[0][u & 1]));
+        mma_commit_elect(smem_u32(&bars.free[slot]));
+        if (t + 2 < nb) issue_s();
+      }
+    }
+    // nothing of this CTA may still be running on the tensor cores when tensor memory is freed
+    mma_commit_elect(smem_u32(&bars.drain[0]));
+    mbar_wait_drain(smem_u32(&bars.drain[0]), 0);
+  } else if (warp == kSoftWarps + 1) {
+    fetch_blocks<D, KK, kSlots>(P, A, tmKc, tmVc, tmK, tmV, walk, sRing, bars, lane, &abort_flag);
+  } else {
+    mend_blocks<D, KK, kSlots>(P, walk, sRing, bars, odd_values, lane, &abort_flag);
+  }
+
+  tc_fence_before_sync();
+  __syncthreads();
+  if (warp == kSoftWarps) tmem_dealloc(tm, 256);
   if (tid == 0 && abort_flag && P.status != nullptr) atomicOr(P.status, 1);
 }
 
@@ -994,8 +1318,8 @@ static TreePlan plan_tree(const TreeParams& P, int dtype, int impl) {
   p.tensor_cores = impl != NSA_IMPL_SIMT && tc_serves(P, dtype);
   int64_t ctas = num_sms();
   if (p.tensor_cores) {
-    p.RT = rows <= 32 ? 32 : rows <= 64 ? 64 : rows <= 128 ? 128 : 256;
-    p.KB = tree_tc::keys(p.RT <= 128 ? 1 : 2);
+    p.RT = rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : rows <= 128 ? 128 : 256;
+    p.KB = p.RT <= 64 ? tree_few::KK : tree_tc::keys(p.RT <= 128 ? 1 : 2);
   } else {
     p.RT = rows <= 8 ? 8 : 32;
     p.KB = tree_simt::kKeys;
@@ -1078,28 +1402,42 @@ static int make_tree_map(CUtensorMap* map, const RowView& r, int B, int H, int64
   return encode_bf16_tiles(map, r.p, dims, strides, box);
 }
 
-template <int D, int STREAMS, int SPLIT>
-static int run_tc(const TreeParams& P, const TreePlan& p, cudaStream_t stream) {
-  using S = tree_tc::Shape<D, STREAMS>;
+// The kernel with its tensor maps, for blocks of KEYS keys, then the merge
+template <auto Kernel, int D, int RT, int KEYS>
+static int run_tiles(const TreeParams& P, const TreePlan& p, int threads, int smem, cudaStream_t stream) {
   CUtensorMap tmKc, tmVc, tmK, tmV;
   TreeAxes A = {};
-  int rc = make_tree_map(&tmK, P.k, P.batch, P.kv_heads, P.tokens, P.d, S::KK, &A.k_b, &A.k_h);
-  if (rc == NSA_OK) rc = make_tree_map(&tmV, P.v, P.batch, P.kv_heads, P.tokens, P.d, S::KK, &A.v_b, &A.v_h);
+  int rc = make_tree_map(&tmK, P.k, P.batch, P.kv_heads, P.tokens, P.d, KEYS, &A.k_b, &A.k_h);
+  if (rc == NSA_OK) rc = make_tree_map(&tmV, P.v, P.batch, P.kv_heads, P.tokens, P.d, KEYS, &A.v_b, &A.v_h);
   tmKc = tmK; tmVc = tmV;                 // an empty cache is never looked at
-  if (rc == NSA_OK && P.capacity > 0) rc = make_tree_map(&tmKc, P.kc, P.batch, P.kv_heads, P.capacity, P.d, S::KK, &A.kc_b, &A.kc_h);
-  if (rc == NSA_OK && P.capacity > 0) rc = make_tree_map(&tmVc, P.vc, P.batch, P.kv_heads, P.capacity, P.d, S::KK, &A.vc_b, &A.vc_h);
+  if (rc == NSA_OK && P.capacity > 0) rc = make_tree_map(&tmKc, P.kc, P.batch, P.kv_heads, P.capacity, P.d, KEYS, &A.kc_b, &A.kc_h);
+  if (rc == NSA_OK && P.capacity > 0) rc = make_tree_map(&tmVc, P.vc, P.batch, P.kv_heads, P.capacity, P.d, KEYS, &A.vc_b, &A.vc_h);
   if (rc != NSA_OK) return rc;
   const int q_vec = (reinterpret_cast<uintptr_t>(P.q.p) & 15u) == 0 && P.q.sb % 8 == 0 && P.q.sh % 8 == 0 && P.q.sn % 8 == 0;
-  TREE_TRY((allow_shared_memory<tree_tc_kernel<D, STREAMS, SPLIT>>()));
-  tree_tc_kernel<D, STREAMS, SPLIT><<<(unsigned)(p.groups * p.tiles), S::kThreads, S::kBytes, stream>>>(tmKc, tmVc, tmK, tmV, P, A, q_vec);
-  return run_merge<__nv_bfloat16, D, STREAMS * tree_tc::kRows / SPLIT, S::KK>(P, p, stream);
+  TREE_TRY(allow_shared_memory<Kernel>());
+  Kernel<<<(unsigned)(p.groups * p.tiles), threads, smem, stream>>>(tmKc, tmVc, tmK, tmV, P, A, q_vec);
+  return run_merge<__nv_bfloat16, D, RT, KEYS>(P, p, stream);
+}
+
+template <int D, int STREAMS>
+static int run_tc(const TreeParams& P, const TreePlan& p, cudaStream_t stream) {
+  using S = tree_tc::Shape<D, STREAMS>;
+  return run_tiles<tree_tc_kernel<D, STREAMS>, D, STREAMS * tree_tc::kRows, S::KK>(P, p, S::kThreads, S::kBytes, stream);
+}
+template <int D, int N>
+static int run_few(const TreeParams& P, const TreePlan& p, cudaStream_t stream) {
+  return run_tiles<tree_few_kernel<D, N>, D, N, tree_few::KK>(P, p, tree_few::Shape<D, N>::kThreads, tree_few::Shape<D, N>::kBytes, stream);
 }
 
 template <int D>
 static int run_tc_rows(const TreeParams& P, const TreePlan& p, cudaStream_t stream) {
-  if (p.RT == 32) return run_tc<D, 1, 4>(P, p, stream);
-  if (p.RT == 64) return run_tc<D, 1, 2>(P, p, stream);
-  return p.RT == 128 ? run_tc<D, 1, 1>(P, p, stream) : run_tc<D, 2, 1>(P, p, stream);
+  switch (p.RT) {
+    case 16: return run_few<D, 16>(P, p, stream);
+    case 32: return run_few<D, 32>(P, p, stream);
+    case 64: return run_few<D, 64>(P, p, stream);
+    case 128: return run_tc<D, 1>(P, p, stream);
+    default: return run_tc<D, 2>(P, p, stream);
+  }
 }
 
 int launch_tree(TreeParams& P, int dtype, int impl, uint8_t* workspace, cudaStream_t stream) {
