@@ -19,23 +19,19 @@
 
 namespace nsa {
 
-#ifndef HEADS_MB
-#define HEADS_MB 4
-#define HEADS_HN 1
-#define HEADS_HB 4
-#define HEADS_PER 32
-#define HEADS_W 6
-#define HEADS_R 8
-#define HEADS_ST 5
-#define HEADS_STB 3
-#define HEADS_MR 4
-#endif
 namespace heads {
 
-#ifndef HEADS_T
-#define HEADS_T 128
-#endif
-constexpr int kThreads = HEADS_T;
+// 128 threads, four blocks an SM: the registers for sixteen values, their factors and four rows under way (256 and two: 65536 x 72 heads
+// of 128 368 instead of 365 us, the gradients of 3063 x 10 of 80 36 instead of 27, for their fewer blocks).
+constexpr int kThreads = 128, kBlocksPerSM = 4;
+// Heads of a slot: angles are formed once for them (8: 16383 x 72 heads of 128 117 us, 32: 102).
+constexpr int kMostHeads = 32;
+// Few tokens: slots are cut until there are this many blocks for each of the 148 SMs (twelve: 2 x 16384 x 20 heads of 64 86 us, six: 67).
+constexpr int kEnoughBlocks = 6;
+// Partial weight gradients come from this many blocks for each SM: twice what is resident, so that the last ones even out (four: 161 us
+// for 4 x 8192 x 36 heads of 64 with gradients, eight: 152, sixteen: 155).
+constexpr int kPartialBlocks = 8;
+constexpr int kSMs = 148;
 enum { kNone = 0, kShared = 1, kPerHead = 2 };
 
 template <int BYTES> struct RawOf;
@@ -221,7 +217,7 @@ __device__ __forceinline__ float row_sum(float v, int lanes) {
 // WEIGHTS: kNone (no norm), kShared, kPerHead
 // FULL: every lane has both vectors of every unit
 template <typename T, int W, int UPL, bool HALF, int WEIGHTS, bool BWD, bool FULL>
-__global__ void __launch_bounds__(heads::kThreads, FULL && WEIGHTS != heads::kNone ? HEADS_MR : HEADS_MB) heads_kernel(const HeadsParams P) {
+__global__ void __launch_bounds__(heads::kThreads, heads::kBlocksPerSM) heads_kernel(const HeadsParams P) {
   using namespace heads;
   using V = Vec<T, W>;
   typedef typename V::Raw Raw;
@@ -230,8 +226,8 @@ __global__ void __launch_bounds__(heads::kThreads, FULL && WEIGHTS != heads::kNo
   constexpr bool FOLD = WEIGHTS == kShared && !BWD;               // the weights are part of the rotation's factors
   constexpr bool ONE = WEIGHTS == kPerHead && BWD;                // one head a slot, whose weight gradient stays in registers
   constexpr bool RING = FULL && NORM;                             // rows come through shared memory
-  constexpr int kVecs = BWD ? 4 : 2, kStages = RING ? (BWD ? HEADS_STB : HEADS_ST) : 1;
-  constexpr int kBatch = UPL > 1 || ONE || RING ? 1 : (BWD && NORM ? HEADS_HN : HEADS_HB);     // heads in flight
+  constexpr int kVecs = BWD ? 4 : 2, kStages = RING ? (BWD ? 3 : 5) : 1;     // (three forward: 111 us for 16383 x 72 heads of 128, five: 103)
+  constexpr int kBatch = UPL > 1 || RING || (BWD && NORM) ? 1 : 4;     // heads in flight, in registers (two for 65536 x 72 of 128: 390 us, four: 369)
   constexpr int FIRST = first_pairs<W, HALF>();
   __shared__ float fold[NORM && BWD ? kThreads / 32 : 1][NORM && BWD ? kHeadsMaxDim : 1];
   __shared__ __align__(16) float held[NORM && BWD ? 32 * UPL : 1][NORM && BWD ? 2 * W : 1];   // the backward's weights, unit by unit
@@ -550,16 +546,17 @@ static int vector_width(const HeadsParams& P, int size, bool backward) {
 
 // Heads a slot, and blocks over the tokens for the slots of the queries and of the keys.  `one`: a head a slot.
 static int heads_grid(HeadsParams& P, bool persistent, bool one, int groups) {
+  using namespace heads;
   const int64_t all = ((int64_t)P.batch * P.seq + groups - 1) / groups;
-  int per = one ? 1 : HEADS_PER;
+  int per = one ? 1 : kMostHeads;
   auto slots = [&](int p) { return (int64_t)(P.part[0].heads + p - 1) / p + (P.part[1].heads + p - 1) / p; };
   // one set of angles serves a slot's heads; few tokens: heads go to blocks of their own until every SM has several
-  while (per > 1 && all * slots(per) < (persistent ? HEADS_R : HEADS_W) * 148) per /= 2;
+  while (per > 1 && all * slots(per) < (persistent ? kPartialBlocks : kEnoughBlocks) * kSMs) per /= 2;
   int64_t total = 0;
   for (int i = 0; i < 2; ++i) {
     P.slots[i] = (P.part[i].heads + per - 1) / per;
-    // with partial weight gradients as many blocks as are resident at once, by the parts' share of the heads
-    const int64_t share = (int64_t)HEADS_R * 148 * P.part[i].heads / (P.part[0].heads + P.part[1].heads);
+    // with partial weight gradients a set number of blocks, by the parts' share of the heads
+    const int64_t share = (int64_t)kPartialBlocks * kSMs * P.part[i].heads / (P.part[0].heads + P.part[1].heads);
     const int64_t most = P.slots[i] > 0 ? (share + P.slots[i] - 1) / P.slots[i] : 1;
     const int64_t blocks = persistent && all > most ? (most > 0 ? most : 1) : all;
     if (blocks > 0x7fffffffLL) return fail(NSA_ERR_SHAPE, "heads: too many tokens for one launch");
@@ -582,7 +579,7 @@ static int lane_shift(const HeadsParams& P, int W, int* units_per_lane) {
 int64_t heads_partial_floats(const HeadsParams& P0) {
   if (!P0.norm) return 0;
   // blocks: the share of each part, rounded up once for each slot
-  return (HEADS_R * 148 + 2 * ((int64_t)P0.part[0].heads + P0.part[1].heads)) * P0.d;
+  return (heads::kPartialBlocks * heads::kSMs + 2 * ((int64_t)P0.part[0].heads + P0.part[1].heads)) * P0.d;
 }
 
 template <typename T, int W, int UPL, int WEIGHTS, bool BWD>

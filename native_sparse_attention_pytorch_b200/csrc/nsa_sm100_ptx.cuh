@@ -374,38 +374,19 @@ __device__ __forceinline__ float exp_row32(float (&s)[32], float scale_log2, flo
 }
 // The same, rounded to bf16 pairs as the A operand in tensor memory holds them (element 2c in the low half of r[c]).  Sums and
 // roundings follow the exponentials at a distance of eight values: a warp issues in order, and what waits for an exponential holds
-// up the next.  SHARE of every 16 values go to the multiplying units instead of the exponential unit, which takes eight cycles for a
-// warp's 32: 2^x = 2^n 2^f with n the nearest whole number (by adding 1.5 * 2^23, + 127 so that the low bits are n's exponent) and
-// |f| <= 1/2, 2^f by its polynomial of degree 4 with the least relative error (2.7e-6 in fp32; found by the Remez exchange).  Below
-// 2^-126 a value counts as that (so SHARE > 0 is for rows without masked logits); NaN stays.
-template <int N, int SHARE>
-__device__ __forceinline__ float exp_pack_row(float (&s)[N], float scale_log2, float off, uint32_t (&r)[N / 2]) {
-  constexpr float kMagic = 12582912.f + 127.f;
-  constexpr int kBehind = 8;
+// up the next.  (64 values: 612 cycles, 512 of them the exponential unit's.  A quarter or three eighths of them as polynomials on the
+// multiplying units took the kernels' clock down with the power: 508 -> 513 to 545 us for 64 tokens over 65536 rows.)
+__device__ __forceinline__ float exp_pack_row(float (&s)[32], float scale_log2, float off, uint32_t (&r)[16]) {
+  constexpr int N = 32, kBehind = 8;
   const uint64_t scale2 = pack2(scale_log2, scale_log2), off2 = pack2(-off, -off);
-  const uint64_t magic = pack2(kMagic, kMagic), less = pack2(-kMagic, -kMagic), minus = pack2(-1.f, -1.f);
-  const uint64_t c0 = pack2(0.9999992847442627f, 0.9999992847442627f), c1 = pack2(0.6931217908859253f, 0.6931217908859253f),
-                 c2 = pack2(0.240247443318367f, 0.240247443318367f), c3 = pack2(0.05591785907745361f, 0.05591785907745361f),
-                 c4 = pack2(0.009570102207362652f, 0.009570102207362652f);
   uint64_t l0 = 0ull, l1 = 0ull;
 #pragma unroll
   for (int x = 0; x < N; x += 2) unpack2(fma2(pack2(s[x], s[x + 1]), scale2, off2), s[x], s[x + 1]);
 #pragma unroll
   for (int x = 0; x < N + kBehind; x += 2) {
     if (x < N) {
-      if (x % 16 < 16 - SHARE) {
-        s[x] = ex2(s[x]);
-        s[x + 1] = ex2(s[x + 1]);
-      } else {
-        float a, b;
-        asm("max.NaN.f32 %0, %1, 0fC2FC0000;" : "=f"(a) : "f"(s[x]));          // -126
-        asm("max.NaN.f32 %0, %1, 0fC2FC0000;" : "=f"(b) : "f"(s[x + 1]));
-        const uint64_t y = pack2(a, b), t = add2(y, magic), f = fma2(add2(t, less), minus, y);
-        const uint64_t p = fma2(fma2(fma2(fma2(c4, f, c3), f, c2), f, c1), f, c0);
-        float ta, tb;
-        unpack2(t, ta, tb);
-        unpack2(mul2(p, pack2(__uint_as_float(__float_as_uint(ta) << 23), __uint_as_float(__float_as_uint(tb) << 23))), s[x], s[x + 1]);
-      }
+      s[x] = ex2(s[x]);
+      s[x + 1] = ex2(s[x + 1]);
     }
     if (x >= kBehind) {
       const int y = x - kBehind;
@@ -419,7 +400,7 @@ __device__ __forceinline__ float exp_pack_row(float (&s)[N], float scale_log2, f
   unpack2(l1, c, d);
   return (a + b) + (c + d);
 }
-// 16 or 8 columns of such pairs of the lane's row
+// 16 columns of such pairs of the lane's row
 __device__ __forceinline__ void tmem_st_words(uint32_t taddr, const uint32_t (&r)[16]) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
@@ -427,11 +408,6 @@ __device__ __forceinline__ void tmem_st_words(uint32_t taddr, const uint32_t (&r
       ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
         "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
       : "memory");
-}
-__device__ __forceinline__ void tmem_st_words(uint32_t taddr, const uint32_t (&r)[8]) {
-  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
-               ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
-               : "memory");
 }
 __device__ __forceinline__ void red_add_v4(float* addr, float a, float b, float c, float d) {
   asm volatile("red.global.add.v4.f32 [%0], {%1, %2, %3, %4};" ::"l"(addr), "f"(a), "f"(b), "f"(c), "f"(d) : "memory");

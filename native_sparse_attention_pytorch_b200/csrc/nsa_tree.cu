@@ -101,22 +101,21 @@ __device__ __forceinline__ bool sees(const TreeParams& P, int b, int t, int u) {
   return P.mask != nullptr ? P.mask[b * P.m_sb + t * P.m_st + u] != 0 : u <= t;
 }
 
-// Which of N drafted rows from `first` on token t sees, and which of N rows (token, head) from `first` on see drafted row u: bits.  The
-// loads do not depend on one another, so that they are under way all at once.
-template <int N>
-__device__ __forceinline__ uint32_t seen_from(const TreeParams& P, int b, int t, int first) {
+// Which of 32 drafted rows from `first` on token t sees, `row` its row of the mask (or NULL); and which of N rows (token, head) from
+// `first` on see drafted row u: bits.  The loads do not depend on one another, so that they are under way all at once; a call of its
+// own, because they would take registers from the loop over the cached keys.
+__device__ __noinline__ uint32_t seen_from(const uint8_t* row, int t, int first, int tokens) {
   uint32_t bits = 0;
-  if (P.mask == nullptr) {
+  if (row == nullptr) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) bits |= (first + i <= t && first + i < P.tokens ? 1u : 0u) << i;
+    for (int i = 0; i < 32; ++i) bits |= (first + i <= t ? 1u : 0u) << i;
     return bits;
   }
-  const uint8_t* m = P.mask + b * P.m_sb + t * P.m_st;
-  uint8_t v[N];
+  uint8_t v[32];
 #pragma unroll
-  for (int i = 0; i < N; ++i) v[i] = m[min(first + i, P.tokens - 1)];
+  for (int i = 0; i < 32; ++i) v[i] = row[min(first + i, tokens - 1)];
 #pragma unroll
-  for (int i = 0; i < N; ++i) bits |= (v[i] != 0 && first + i < P.tokens ? 1u : 0u) << i;
+  for (int i = 0; i < 32; ++i) bits |= (v[i] != 0 && first + i < tokens ? 1u : 0u) << i;
   return bits;
 }
 template <int N>
@@ -394,10 +393,6 @@ __global__ void __launch_bounds__(tree_simt::kThreads, 2) tree_simt_kernel(const
 // STREAMS.  Above 128 rows two tiles share the K and V blocks; the softmax of one runs under the products of the other.  Blocks of 64
 // keys, so that tensor memory holds two S buffers of either beside both O: with blocks of 128 and one buffer, S of the next block
 // waited for the products of this one, which waited for its softmax (3800 cycles a block and pair of tiles, 2050 of them products).
-#ifndef TREE_SHARE
-#define TREE_SHARE 0
-#define TREE_TURNS 1
-#endif
 namespace tree_tc {
 constexpr int kRows = 128;
 constexpr int keys(int streams) { return streams == 1 ? 128 : 64; }     // of a block
@@ -645,7 +640,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmKc, const __grid_constant__
     const bool working = s < streams && local - lane < here;
     // Two streams: the two warps of a quarter, which share an exponential unit, take turns at it, so that one's maxima, waits and
     // transfers fall into the other's exponentials
-    const bool turns = TREE_TURNS && STREAMS == 2 && row0 + kRows + quarter * 32 < rows;
+    const bool turns = STREAMS == 2 && row0 + kRows + quarter * 32 < rows;
     auto my_turn = [&]() { asm volatile("bar.sync %0, 64;" ::"r"(1 + s * 4 + quarter) : "memory"); };
     auto your_turn = [&]() { asm volatile("bar.arrive %0, 64;" ::"r"(1 + (s ^ 1) * 4 + quarter) : "memory"); };
     uint32_t u = 0;
@@ -687,13 +682,10 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmKc, const __grid_constant__
           tmem_ld32(tS + half * CW + k * 32, x[k]);
         }
         tmem_ld_wait();
-        const bool masked = draft || n < CW;
         if (draft) {
 #pragma unroll
           for (int k = 0; k < NCH; ++k) {
-            uint32_t seen = 0;
-#pragma unroll 1
-            for (int i = 0; valid && i < CH; i += 8) seen |= seen_from<8>(P, walk.b, t, first + k * CH + i) << i;
+            const uint32_t seen = valid ? seen_from(P.mask != nullptr ? P.mask + walk.b * P.m_sb + t * P.m_st : nullptr, t, first + k * CH, P.tokens) : 0;
 #pragma unroll
             for (int i = 0; i < CH; ++i)
               if (!(seen >> i & 1)) x[k][i] = -INFINITY;
@@ -744,8 +736,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmKc, const __grid_constant__
 #pragma unroll
         for (int k = 0; k < NCH; ++k) {
           uint32_t r[CH / 2];
-          if (masked) l += exp_pack_row<CH, 0>(x[k], scale2, ref, r);       // a masked logit, -inf, gives 0
-          else l += exp_pack_row<CH, TREE_SHARE>(x[k], scale2, ref, r);
+          l += exp_pack_row(x[k], scale2, ref, r);       // a masked logit, -inf, gives 0
           if (STREAMS == 2 && turns && k == NCH - 1) your_turn();
           tmem_st_words(tP + half * (CW / 2) + k * 16, r);
         }
