@@ -108,18 +108,29 @@ __device__ __forceinline__ void split(const typename Vec<T, W>::Raw& a, const ty
     }
   }
 }
-// A unit's weights, of head h where there is a row per head
+// A unit's weights, of head h where there is a row per head (rows lie on the vectors' boundaries, see vector_width)
 template <typename T, int W, bool HALF>
 __device__ __forceinline__ void load_weight(const HeadsParams& P, const HeadRows& R, const Unit& t, int h, float* wu, float* wv) {
   const int64_t row = P.weight_per_head ? (int64_t)h * P.d : 0;
-  auto weight = [&](int e) { return P.weight_f32 ? __ldg((const float*)R.weight + row + e) : Elem<T>::to_float(((const T*)R.weight)[row + e]); };
+  float x[W], y[W];
+  auto vector = [&](int at, float* out) {
+#pragma unroll
+    for (int i = 0; i < W; ++i) out[i] = 0.f;
+    if (at < 0) return;
+    if (!P.weight_f32) {
+      Vec<T, W>::widen(Vec<T, W>::load((const T*)R.weight + row + at), out);
+    } else {
+      constexpr int F = W < 4 ? W : 4;
+#pragma unroll
+      for (int i = 0; i < W; i += F) Vec<float, F>::widen(Vec<float, F>::load((const float*)R.weight + row + at + i), out + i);
+    }
+  };
+  vector(t.a, x);
+  vector(t.b, y);
 #pragma unroll
   for (int i = 0; i < W; ++i) {
-    const bool second = !HALF && W > 1 && 2 * i >= W;
-    const int at = HALF || W == 1 ? t.a : (second ? t.b : t.a);
-    const int eu = HALF || W == 1 ? t.a + i : at + (2 * i) % W, ev = HALF || W == 1 ? t.b + i : eu + 1;
-    wu[i] = at < 0 ? 0.f : weight(eu);
-    wv[i] = (HALF || W == 1 ? t.b : at) < 0 ? 0.f : weight(ev);
+    wu[i] = HALF || W == 1 ? x[i] : (2 * i < W ? x[(2 * i) % W] : y[(2 * i) % W]);
+    wv[i] = HALF || W == 1 ? y[i] : (2 * i < W ? x[(2 * i + 1) % W] : y[(2 * i + 1) % W]);
   }
 }
 template <typename T, int W, bool HALF, bool FULL>
@@ -537,6 +548,10 @@ static int vector_width(const HeadsParams& P, int size, bool backward) {
   for (const HeadRows& r : P.part) {
     if (r.heads == 0) continue;
     all |= reinterpret_cast<uintptr_t>(r.out) | (uint64_t)(r.o_sb | r.o_sh | r.o_sn) * size;
+    if (P.norm) {        // fp32 weights are read four at a time beside bf16 rows
+      const uintptr_t at = reinterpret_cast<uintptr_t>(r.weight) & 15;
+      all |= P.weight_f32 && size == 2 ? (at & 4 ? 2 : at & 8 ? 4 : 0) : at;
+    }
     if (r.x != nullptr) all |= reinterpret_cast<uintptr_t>(r.x) | (uint64_t)(r.x_sb | r.x_sh | r.x_sn) * size;
     if (backward) all |= reinterpret_cast<uintptr_t>(r.dy) | (uint64_t)(r.dy_sb | r.dy_sh | r.dy_sn) * size;
   }
@@ -624,6 +639,7 @@ static int launch_heads_typed(HeadsParams& P, cudaStream_t stream) {
   const int W = vector_width(P, sizeof(T), BWD);
   if (W >= kMost) return launch_heads_w<T, kMost, 1, WEIGHTS, BWD>(P, stream);
   if (W >= kMost / 2) return launch_heads_w<T, kMost / 2, kMost / 2 >= 4 ? 1 : 2, WEIGHTS, BWD>(P, stream);
+  if (kMost / 4 > 1 && W >= kMost / 4) return launch_heads_w<T, kMost / 4 < 2 ? 2 : kMost / 4, 2, WEIGHTS, BWD>(P, stream);
   return launch_heads_w<T, 1, 4, WEIGHTS, BWD>(P, stream);
 }
 

@@ -154,14 +154,16 @@ __device__ __forceinline__ const T* row_of(const RowView& r, int b, int h, int64
 // ---- any type and alignment, on the CUDA cores -------------------------------------------
 
 namespace tree_simt {
-constexpr int kKeys = 64, kThreads = 256;
+constexpr int kThreads = 256;
 template <int DP, int RT>
 struct Shape {
+  static constexpr int kKeys = RT == 64 ? 32 : 64;          // of a block: two CTAs' tiles fit an SM
   static constexpr int kRow = DP + 4;                       // padded: four neighbouring rows on different banks
   static constexpr int kScore = kKeys + 4;
-  static constexpr int TX = RT == 32 ? 16 : 64, TY = kThreads / TX;
+  static constexpr int TX = RT == 8 ? 64 : 16, TY = kThreads / TX;
   static constexpr int KPT = kKeys / TX, RPT = RT / TY;     // keys and rows of a thread
-  static constexpr int CPT = DP / TX;                       // output columns of a thread
+  static constexpr int CPT = DP / TX;                       // output columns of a thread, VC neighbours every VC TX
+  static constexpr int VC = CPT < 4 ? CPT : 4;
   static constexpr int kFloats = RT * kRow + 2 * kKeys * kRow + RT * kScore + 3 * RT;
 };
 }  // namespace tree_simt
@@ -172,7 +174,7 @@ __global__ void __launch_bounds__(tree_simt::kThreads, 2) tree_simt_kernel(const
   using namespace tree;
   using namespace tree_simt;
   using S = Shape<DP, RT>;
-  constexpr int V = 16 / (int)sizeof(T);
+  constexpr int V = 16 / (int)sizeof(T), kKeys = S::kKeys;
   extern __shared__ __align__(16) float tree_smem[];
   float* const qs = tree_smem;
   float* const ks = qs + RT * S::kRow;
@@ -184,6 +186,7 @@ __global__ void __launch_bounds__(tree_simt::kThreads, 2) tree_simt_kernel(const
   __shared__ int odd_values;       // a drafted value of this unit is not finite
   const int tid = threadIdx.x, lane = tid & 31;
   const int tx = tid % S::TX, ty = tid / S::TX;
+  auto column = [&](int c) { return (c / S::VC * S::TX + tx) * S::VC + c % S::VC; };
   const int tile = blockIdx.x % P.tiles, group = blockIdx.x / P.tiles;
   const int rows = P.tokens * P.G, row0 = tile * RT;
 
@@ -311,23 +314,40 @@ __global__ void __launch_bounds__(tree_simt::kThreads, 2) tree_simt_kernel(const
       }
       __syncthreads();
 
-      // output columns tx CPT + c
+      // output columns: column(c)
 #pragma unroll
       for (int r = 0; r < S::RPT; ++r) {
         const float a = row_a[ty * S::RPT + r];
 #pragma unroll
         for (int c = 0; c < S::CPT; ++c) o[r][c] *= a;
       }
-#pragma unroll 4
-      for (int k = 0; k < kKeys; ++k) {
-        float p[S::RPT];
+#pragma unroll 2
+      for (int k = 0; k < kKeys; k += 4) {
+        float4 p[S::RPT];
 #pragma unroll
-        for (int r = 0; r < S::RPT; ++r) p[r] = ss[(ty * S::RPT + r) * S::kScore + k];
+        for (int r = 0; r < S::RPT; ++r) p[r] = *reinterpret_cast<const float4*>(ss + (ty * S::RPT + r) * S::kScore + k);
 #pragma unroll
-        for (int c = 0; c < S::CPT; ++c) {
-          const float v = vs[k * S::kRow + tx * S::CPT + c];
+        for (int kk = 0; kk < 4; ++kk) {
+          float v[S::CPT];
 #pragma unroll
-          for (int r = 0; r < S::RPT; ++r) o[r][c] += p[r] * v;
+          for (int c = 0; c < S::CPT; c += S::VC) {
+            const float* at = vs + (k + kk) * S::kRow + column(c);
+            if constexpr (S::VC == 4) {
+              const float4 q = *reinterpret_cast<const float4*>(at);
+              v[c] = q.x; v[c + 1] = q.y; v[c + 2] = q.z; v[c + 3] = q.w;
+            } else if constexpr (S::VC == 2) {
+              const float2 q = *reinterpret_cast<const float2*>(at);
+              v[c] = q.x; v[c + 1] = q.y;
+            } else {
+              v[c] = *at;
+            }
+          }
+#pragma unroll
+          for (int r = 0; r < S::RPT; ++r) {
+            const float w = kk == 0 ? p[r].x : kk == 1 ? p[r].y : kk == 2 ? p[r].z : p[r].w;
+#pragma unroll
+            for (int c = 0; c < S::CPT; ++c) o[r][c] += w * v[c];
+          }
         }
       }
     }
@@ -341,7 +361,7 @@ __global__ void __launch_bounds__(tree_simt::kThreads, 2) tree_simt_kernel(const
           if (row >= rows || !sees(P, at.b, row / P.G, u)) continue;
 #pragma unroll
           for (int c = 0; c < S::CPT; ++c) {
-            const int col = tx * S::CPT + c;
+            const int col = column(c);
             const float v = col < P.d ? Elem<T>::to_float(row_of<T>(P.v, at.b, h, u)[col]) : 0.f;
             if (!isfinite(v)) o[r][c] += v;
           }
@@ -361,12 +381,12 @@ __global__ void __launch_bounds__(tree_simt::kThreads, 2) tree_simt_kernel(const
         const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);      // a sum that is NaN stays NaN
 #pragma unroll
         for (int c = 0; c < S::CPT; ++c)
-          if (tx * S::CPT + c < P.d) out[tx * S::CPT + c] = Elem<T>::from_float(o[r][c] * inv);
+          if (column(c) < P.d) out[column(c)] = Elem<T>::from_float(o[r][c] * inv);
         if (tx == 0 && P.lse != nullptr)
           P.lse[((int64_t)at.b * P.q_heads + h * P.G + g) * P.tokens + t] = l == 0.f ? -INFINITY : (row_m[local] + log2f(l)) * kLn2;
       } else {
 #pragma unroll
-        for (int c = 0; c < S::CPT; ++c) P.partial[(slot * RT + local) * DP + tx * S::CPT + c] = o[r][c];
+        for (int c = 0; c < S::CPT; ++c) P.partial[(slot * RT + local) * DP + column(c)] = o[r][c];
         if (tx == 0) P.stats[slot * RT + local] = make_float2(row_m[local], l);
       }
     }
@@ -873,7 +893,8 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmKc, const __grid_constant__
 //     and those of the drafted rows, the maxima are taken, O^T and the sums rescaled.
 //   * Sums stay with the threads, a key each, until a unit ends.
 //   * The transposed accumulator leaves whole rows of the output side by side.
-// Against the tile with rows as rows and copies of them over the keys: XXX
+// Against the tile with rows as rows and copies of them over the keys, calls back to back: one token over 4096 rows 12.3 -> 11.6 us, 32
+// x one token over 16384 (64 / 8 heads of 128) 248 -> 244 us, 8 x 16 tokens over 16384 (16 / 4 heads of 64) 39 us either way.
 namespace tree_few {
 constexpr int KK = 128;
 template <int D, int N>
@@ -1232,8 +1253,8 @@ __global__ void __launch_bounds__(256) tree_merge_kernel(const TreeParams P) {
   const int per_unit = cache_blocks<KB>(P, b) + draft_blocks<KB>(P);
   const int64_t unit0 = before + (int64_t)h * per_unit;
   const int g0 = group_of(total, unit0, groups), g1 = group_of(total, unit0 + per_unit - 1, groups);
+  ptx::grid_wait();                          // on every path: what follows in the stream waits for this kernel alone
   if (g0 == g1) return;                      // written as a whole (the same for all of a block)
-  ptx::grid_wait();
   const bool there = row < rows;
   const int tile = (there ? row : 0) / RT, local = (there ? row : 0) - tile * RT;
   auto slot_of = [&](int g) { return ((int64_t)g * P.tiles + tile) * 2 + (g == g0 ? 1 : 0); };
@@ -1312,8 +1333,8 @@ static TreePlan plan_tree(const TreeParams& P, int dtype, int impl) {
     p.RT = rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : rows <= 128 ? 128 : 256;
     p.KB = p.RT <= 64 ? tree_few::KK : tree_tc::keys(p.RT <= 128 ? 1 : 2);
   } else {
-    p.RT = rows <= 8 ? 8 : 32;
-    p.KB = tree_simt::kKeys;
+    p.RT = rows <= 8 ? 8 : rows <= 32 ? 32 : 64;
+    p.KB = p.RT == 64 ? 32 : 64;
     ctas *= 2;
   }
   p.tiles = (int)((rows + p.RT - 1) / p.RT);
@@ -1372,13 +1393,16 @@ static int run_simt(const TreeParams& P, const TreePlan& p, cudaStream_t stream)
   const int smem = tree_simt::Shape<DP, RT>::kFloats * (int)sizeof(float);
   TREE_TRY((allow_shared_memory<tree_simt_kernel<T, DP, RT>>()));
   tree_simt_kernel<T, DP, RT><<<(unsigned)(p.groups * p.tiles), tree_simt::kThreads, smem, stream>>>(P, vec);
-  return run_merge<T, DP, RT, tree_simt::kKeys>(P, p, stream);
+  return run_merge<T, DP, RT, tree_simt::Shape<DP, RT>::kKeys>(P, p, stream);
 }
 
 template <typename T>
 static int run_simt_typed(const TreeParams& P, const TreePlan& p, cudaStream_t stream) {
-  if (p.DP == 64) return p.RT == 8 ? run_simt<T, 64, 8>(P, p, stream) : run_simt<T, 64, 32>(P, p, stream);
-  return p.RT == 8 ? run_simt<T, 128, 8>(P, p, stream) : run_simt<T, 128, 32>(P, p, stream);
+  switch (p.RT) {
+    case 8: return p.DP == 64 ? run_simt<T, 64, 8>(P, p, stream) : run_simt<T, 128, 8>(P, p, stream);
+    case 32: return p.DP == 64 ? run_simt<T, 64, 32>(P, p, stream) : run_simt<T, 128, 32>(P, p, stream);
+    default: return p.DP == 64 ? run_simt<T, 64, 64>(P, p, stream) : run_simt<T, 128, 64>(P, p, stream);
+  }
 }
 
 // Boxes of 64 features x `rows` rows of one head.  An axis of one entry, or of stride zero, is one entry in the map; `step_b` and
