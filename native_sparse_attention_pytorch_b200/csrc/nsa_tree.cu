@@ -1245,7 +1245,7 @@ __global__ void __launch_bounds__(256) tree_merge_kernel(const TreeParams P) {
   __shared__ __align__(16) float sums[WARPS > 1 ? 8 : 1][DP];
   __shared__ float parts[WARPS > 1 ? 8 : 1];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, part = warp % WARPS;
-  const int rows = P.tokens * P.G, row = blockIdx.x * ROWS + warp / WARPS;
+  const int rows = P.tokens * P.G;
   const int b = blockIdx.y / P.kv_heads, h = blockIdx.y - b * P.kv_heads;
   int64_t before, total;
   count_blocks<KB>(P, lane, b, before, total);
@@ -1255,51 +1255,57 @@ __global__ void __launch_bounds__(256) tree_merge_kernel(const TreeParams P) {
   const int g0 = group_of(total, unit0, groups), g1 = group_of(total, unit0 + per_unit - 1, groups);
   ptx::grid_wait();                          // on every path: what follows in the stream waits for this kernel alone
   if (g0 == g1) return;                      // written as a whole (the same for all of a block)
-  const bool there = row < rows;
-  const int tile = (there ? row : 0) / RT, local = (there ? row : 0) - tile * RT;
-  auto slot_of = [&](int g) { return ((int64_t)g * P.tiles + tile) * 2 + (g == g0 ? 1 : 0); };
+  // (a block's warps stay together: with several of them a row there is a barrier in the loop)
+  for (int row0 = blockIdx.x * ROWS; row0 < rows; row0 += gridDim.x * ROWS) {
+    const int row = row0 + warp / WARPS;
+    const bool there = row < rows;
+    const int tile = (there ? row : 0) / RT, local = (there ? row : 0) - tile * RT;
+    auto slot_of = [&](int g) { return ((int64_t)g * P.tiles + tile) * 2 + (g == g0 ? 1 : 0); };
 
-  float top = -INFINITY;
-  for (int g = g0 + lane; g <= g1; g += 32) top = fmaxf(top, P.stats[slot_of(g) * RT + local].x);
-  top = warp_max(top);
-  const float ref = top == -INFINITY ? 0.f : top;
-  float o[C], l = 0.f;
+    float top = -INFINITY;
+    for (int g = g0 + lane; g <= g1; g += 32) top = fmaxf(top, P.stats[slot_of(g) * RT + local].x);
+    top = warp_max(top);
+    const float ref = top == -INFINITY ? 0.f : top;
+    float o[C], l = 0.f;
 #pragma unroll
-  for (int c = 0; c < C; ++c) o[c] = 0.f;
+    for (int c = 0; c < C; ++c) o[c] = 0.f;
 #pragma unroll 4
-  for (int g = g0 + part; g <= g1; g += WARPS) {
-    const int64_t slot = slot_of(g);
-    const float2 st = P.stats[slot * RT + local];
-    const float w = exp2f(st.x - ref);
-    __align__(16) float v[C];
-    if constexpr (C == 4) *reinterpret_cast<float4*>(v) = *reinterpret_cast<const float4*>(P.partial + (slot * RT + local) * DP + lane * C);
-    else *reinterpret_cast<float2*>(v) = *reinterpret_cast<const float2*>(P.partial + (slot * RT + local) * DP + lane * C);
-    l += st.y * w;
+    for (int g = g0 + part; g <= g1; g += WARPS) {
+      const int64_t slot = slot_of(g);
+      const float2 st = P.stats[slot * RT + local];
+      const float w = exp2f(st.x - ref);
+      __align__(16) float v[C];
+      if constexpr (C == 4) *reinterpret_cast<float4*>(v) = *reinterpret_cast<const float4*>(P.partial + (slot * RT + local) * DP + lane * C);
+      else *reinterpret_cast<float2*>(v) = *reinterpret_cast<const float2*>(P.partial + (slot * RT + local) * DP + lane * C);
+      l += st.y * w;
 #pragma unroll
-    for (int c = 0; c < C; ++c) o[c] += v[c] * w;
-  }
-  if constexpr (WARPS > 1) {
-#pragma unroll
-    for (int c = 0; c < C; ++c) sums[warp][lane * C + c] = o[c];
-    if (lane == 0) parts[warp] = l;
-    __syncthreads();
-    if (part > 0) return;
-#pragma unroll
-    for (int k = 1; k < WARPS; ++k) {
-      l += parts[warp + k];
-#pragma unroll
-      for (int c = 0; c < C; ++c) o[c] += sums[warp + k][lane * C + c];
+      for (int c = 0; c < C; ++c) o[c] += v[c] * w;
     }
-  }
-  if (!there) return;
-  const int t = row / P.G, g = row - t * P.G;
-  const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);      // a sum that is NaN stays NaN
-  T* out = const_cast<T*>(row_of<T>(P.out, b, h * P.G + g, t));
+    if constexpr (WARPS > 1) {
 #pragma unroll
-  for (int c = 0; c < C; ++c)
-    if (lane * C + c < P.d) out[lane * C + c] = Elem<T>::from_float(o[c] * inv);
-  if (lane == 0 && P.lse != nullptr)
-    P.lse[((int64_t)b * P.q_heads + h * P.G + g) * P.tokens + t] = l == 0.f ? -INFINITY : (top + log2f(l)) * kLn2;
+      for (int c = 0; c < C; ++c) sums[warp][lane * C + c] = o[c];
+      if (lane == 0) parts[warp] = l;
+      __syncthreads();
+      if (part == 0) {
+#pragma unroll
+        for (int k = 1; k < WARPS; ++k) {
+          l += parts[warp + k];
+#pragma unroll
+          for (int c = 0; c < C; ++c) o[c] += sums[warp + k][lane * C + c];
+        }
+      }
+      __syncthreads();
+    }
+    if (!there || part > 0) continue;
+    const int t = row / P.G, g = row - t * P.G;
+    const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);      // a sum that is NaN stays NaN
+    T* out = const_cast<T*>(row_of<T>(P.out, b, h * P.G + g, t));
+#pragma unroll
+    for (int c = 0; c < C; ++c)
+      if (lane * C + c < P.d) out[lane * C + c] = Elem<T>::from_float(o[c] * inv);
+    if (lane == 0 && P.lse != nullptr)
+      P.lse[((int64_t)b * P.q_heads + h * P.G + g) * P.tokens + t] = l == 0.f ? -INFINITY : (top + log2f(l)) * kLn2;
+  }
 }
 
 // ---- host ------------------------------------------------------------------------------------
@@ -1361,7 +1367,9 @@ template <typename T, int DP, int RT, int KB, int WARPS>
 static cudaError_t launch_merge(const TreeParams& P, cudaStream_t stream) {
   cudaLaunchConfig_t config = {};
   constexpr int ROWS = 8 / WARPS;
-  config.gridDim = dim3((unsigned)(((int64_t)P.tokens * P.G + ROWS - 1) / ROWS), (unsigned)(P.batch * P.kv_heads));
+  // a block finds its unit's place once for the rows it goes through: no more blocks than are resident at once
+  const int64_t all = ((int64_t)P.tokens * P.G + ROWS - 1) / ROWS, units = (int64_t)P.batch * P.kv_heads, most = (8 * (int64_t)num_sms() + units - 1) / units;
+  config.gridDim = dim3((unsigned)(all < most ? all : most), (unsigned)units);
   config.blockDim = dim3(256);
   config.stream = stream;
   cudaLaunchAttribute overlap = {};
