@@ -157,29 +157,29 @@ namespace tree_simt {
 constexpr int kThreads = 256;
 template <int DP, int RT>
 struct Shape {
-  static constexpr int kKeys = RT == 64 ? 32 : 64;          // of a block: two CTAs' tiles fit an SM
+  static constexpr int kKeys = RT == 8 ? 64 : 32;           // of a block; two are in shared memory
   static constexpr int kRow = DP + 4;                       // padded: four neighbouring rows on different banks
   static constexpr int kScore = kKeys + 4;
   static constexpr int TX = RT == 8 ? 64 : 16, TY = kThreads / TX;
   static constexpr int KPT = kKeys / TX, RPT = RT / TY;     // keys and rows of a thread
   static constexpr int CPT = DP / TX;                       // output columns of a thread, VC neighbours every VC TX
   static constexpr int VC = CPT < 4 ? CPT : 4;
-  static constexpr int kFloats = RT * kRow + 2 * kKeys * kRow + RT * kScore + 3 * RT;
+  static constexpr int kFloats = RT * kRow + 4 * kKeys * kRow + RT * kScore + 3 * RT;
+  static constexpr int kPerSM = kFloats * 4 <= 113 * 1024 ? 2 : 1;          // CTAs
 };
 }  // namespace tree_simt
 
 // DP: dim_head padded to 64 or 128; RT: rows of a tile
 template <typename T, int DP, int RT>
-__global__ void __launch_bounds__(tree_simt::kThreads, 2) tree_simt_kernel(const TreeParams P, const int vec) {
+__global__ void __launch_bounds__(tree_simt::kThreads, tree_simt::Shape<DP, RT>::kPerSM) tree_simt_kernel(const TreeParams P, const int vec) {
   using namespace tree;
   using namespace tree_simt;
   using S = Shape<DP, RT>;
   constexpr int V = 16 / (int)sizeof(T), kKeys = S::kKeys;
   extern __shared__ __align__(16) float tree_smem[];
   float* const qs = tree_smem;
-  float* const ks = qs + RT * S::kRow;
-  float* const vs = ks + kKeys * S::kRow;
-  float* const ss = vs + kKeys * S::kRow;
+  float* const tiles = qs + RT * S::kRow;               // K and V of two blocks
+  float* const ss = tiles + 4 * kKeys * S::kRow;
   float* const row_m = ss + RT * S::kScore;
   float* const row_l = row_m + RT;
   float* const row_a = row_l + RT;
@@ -227,6 +227,18 @@ __global__ void __launch_bounds__(tree_simt::kThreads, 2) tree_simt_kernel(const
     }
   };
 
+  // fp32 rows on 16-byte boundaries come asynchronously, a block ahead
+  const bool ahead = vec && sizeof(T) == 4;
+  auto fetch_rows = [&](float* dst, const T* src, int64_t stride, int n) {
+    const int per = P.d / V;
+    const uint32_t to = ptx::smem_u32(dst);
+    for (int e = tid; e < kKeys * (DP / V); e += kThreads) {
+      const int r = e / (DP / V), c = e - r * (DP / V);
+      const bool there = r < n && c < per;
+      ptx::cp_async16(to + (r * S::kRow + c * V) * 4, there ? src + r * stride + c * V : src, there ? 16 : 0);
+    }
+  };
+
   for (int64_t at_block = begin; at_block < end;) {
     // the unit at_block lies in, and this piece's blocks of it
     const int cached = cache_blocks<kKeys>(P, at.b), per_unit = cached + draft_blocks<kKeys>(P), length = length_of(P, at.b);
@@ -248,12 +260,42 @@ __global__ void __launch_bounds__(tree_simt::kThreads, 2) tree_simt_kernel(const
 #pragma unroll
       for (int c = 0; c < S::CPT; ++c) o[r][c] = 0.f;
 
+    auto fetch_block = [&](int j) {
+      const bool draft = j >= cached;
+      const int first = (draft ? j - cached : j) * kKeys, n = min(kKeys, (draft ? P.tokens : length) - first);
+      float* const to = tiles + (j & 1) * (2 * kKeys * S::kRow);
+      fetch_rows(to, row_of<T>(draft ? P.k : P.kc, at.b, h, first), draft ? P.k.sn : P.kc.sn, n);
+      fetch_rows(to + kKeys * S::kRow, row_of<T>(draft ? P.v : P.vc, at.b, h, first), draft ? P.v.sn : P.vc.sn, n);
+    };
+    if (ahead) {
+      fetch_block(j0);          // (the barrier above: the tiles of the unit before have been read)
+      ptx::cp_async_commit();
+    }
+
     for (int j = j0; j < j1; ++j) {
       const bool draft = j >= cached;
       const int first = (draft ? j - cached : j) * kKeys, n = min(kKeys, (draft ? P.tokens : length) - first);
+      float* const ks = tiles + (j & 1) * (2 * kKeys * S::kRow);
+      float* const vs = ks + kKeys * S::kRow;
       __syncthreads();   // the tiles and scores of the block before have been read
-      load_rows(ks, row_of<T>(draft ? P.k : P.kc, at.b, h, first), draft ? P.k.sn : P.kc.sn, n, kKeys, false);
-      load_rows(vs, row_of<T>(draft ? P.v : P.vc, at.b, h, first), draft ? P.v.sn : P.vc.sn, n, kKeys, draft);
+      if (ahead) {
+        if (j + 1 < j1) fetch_block(j + 1);
+        ptx::cp_async_commit();
+        ptx::cp_async_wait<1>();
+        if (draft) {     // each thread mends what it fetched
+          for (int e = tid; e < kKeys * (DP / V); e += kThreads) {
+            const int r = e / (DP / V), c = e - r * (DP / V);
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+              float& x = vs[r * S::kRow + c * V + i];
+              if (!isfinite(x)) { x = 0.f; odd_values = 1; }
+            }
+          }
+        }
+      } else {
+        load_rows(ks, row_of<T>(draft ? P.k : P.kc, at.b, h, first), draft ? P.k.sn : P.kc.sn, n, kKeys, false);
+        load_rows(vs, row_of<T>(draft ? P.v : P.vc, at.b, h, first), draft ? P.v.sn : P.vc.sn, n, kKeys, draft);
+      }
       __syncthreads();
 
       // scores: keys tx + TX k, rows ty RPT + r
@@ -1340,8 +1382,8 @@ static TreePlan plan_tree(const TreeParams& P, int dtype, int impl) {
     p.KB = p.RT <= 64 ? tree_few::KK : tree_tc::keys(p.RT <= 128 ? 1 : 2);
   } else {
     p.RT = rows <= 8 ? 8 : rows <= 32 ? 32 : 64;
-    p.KB = p.RT == 64 ? 32 : 64;
-    ctas *= 2;
+    p.KB = p.RT == 8 ? 64 : 32;
+    if (p.RT > 8 || p.DP == 64) ctas *= 2;           // Shape::kPerSM
   }
   p.tiles = (int)((rows + p.RT - 1) / p.RT);
   p.groups = p.tiles >= ctas ? 1 : (int)(ctas / p.tiles);
@@ -1398,7 +1440,8 @@ static int run_simt(const TreeParams& P, const TreePlan& p, cudaStream_t stream)
   constexpr int V = 16 / (int)sizeof(T);
   auto wide = [](const RowView& r) { return (reinterpret_cast<uintptr_t>(r.p) & 15u) == 0 && r.sb % V == 0 && r.sh % V == 0 && r.sn % V == 0; };
   const int vec = wide(P.k) && wide(P.v) && (P.capacity == 0 || (wide(P.kc) && wide(P.vc)));
-  const int smem = tree_simt::Shape<DP, RT>::kFloats * (int)sizeof(float);
+  constexpr int smem = tree_simt::Shape<DP, RT>::kFloats * (int)sizeof(float);
+  static_assert(tree_simt::Shape<DP, RT>::kPerSM == (RT > 8 || DP == 64 ? 2 : 1) && smem <= kMaxSharedBytes, "plan_tree");
   TREE_TRY((allow_shared_memory<tree_simt_kernel<T, DP, RT>>()));
   tree_simt_kernel<T, DP, RT><<<(unsigned)(p.groups * p.tiles), tree_simt::kThreads, smem, stream>>>(P, vec);
   return run_merge<T, DP, RT, tree_simt::Shape<DP, RT>::kKeys>(P, p, stream);
