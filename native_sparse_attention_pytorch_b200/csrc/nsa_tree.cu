@@ -1285,7 +1285,7 @@ __global__ void __launch_bounds__(256) tree_merge_kernel(const TreeParams P) {
   using namespace tree;
   constexpr int C = DP / 32, ROWS = 8 / WARPS;
   __shared__ __align__(16) float sums[WARPS > 1 ? 8 : 1][DP];
-  __shared__ float parts[WARPS > 1 ? 8 : 1];
+  __shared__ float2 parts[WARPS > 1 ? 8 : 1];          // maximum, sum
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, part = warp % WARPS;
   const int rows = P.tokens * P.G;
   const int b = blockIdx.y / P.kv_heads, h = blockIdx.y - b * P.kv_heads;
@@ -1304,36 +1304,56 @@ __global__ void __launch_bounds__(256) tree_merge_kernel(const TreeParams P) {
     const int tile = (there ? row : 0) / RT, local = (there ? row : 0) - tile * RT;
     auto slot_of = [&](int g) { return ((int64_t)g * P.tiles + tile) * 2 + (g == g0 ? 1 : 0); };
 
-    float top = -INFINITY;
-    for (int g = g0 + lane; g <= g1; g += 32) top = fmaxf(top, P.stats[slot_of(g) * RT + local].x);
-    top = warp_max(top);
-    const float ref = top == -INFINITY ? 0.f : top;
-    float o[C], l = 0.f;
+    // four partials at a time, statistics and sums of all of them under way together, joined with a running maximum
+    float o[C], l = 0.f, top = -INFINITY;
 #pragma unroll
     for (int c = 0; c < C; ++c) o[c] = 0.f;
-#pragma unroll 4
-    for (int g = g0 + part; g <= g1; g += WARPS) {
-      const int64_t slot = slot_of(g);
-      const float2 st = P.stats[slot * RT + local];
-      const float w = exp2f(st.x - ref);
-      __align__(16) float v[C];
-      if constexpr (C == 4) *reinterpret_cast<float4*>(v) = *reinterpret_cast<const float4*>(P.partial + (slot * RT + local) * DP + lane * C);
-      else *reinterpret_cast<float2*>(v) = *reinterpret_cast<const float2*>(P.partial + (slot * RT + local) * DP + lane * C);
-      l += st.y * w;
+#pragma unroll 1
+    for (int first = g0 + part; first <= g1; first += 4 * WARPS) {
+      float2 st[4];
+      __align__(16) float v[4][C];
 #pragma unroll
-      for (int c = 0; c < C; ++c) o[c] += v[c] * w;
+      for (int k = 0; k < 4; ++k) {
+        const int g = first + k * WARPS;
+        const int64_t at = slot_of(min(g, g1)) * RT + local;      // (the last one again where there are fewer)
+        st[k] = P.stats[at];
+        if constexpr (C == 4) *reinterpret_cast<float4*>(v[k]) = *reinterpret_cast<const float4*>(P.partial + at * DP + lane * C);
+        else *reinterpret_cast<float2*>(v[k]) = *reinterpret_cast<const float2*>(P.partial + at * DP + lane * C);
+      }
+      const float before = top;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) top = fmaxf(top, st[k].x);
+      const float ref = top == -INFINITY ? 0.f : top, a = exp2f(before - ref);
+      l *= a;
+#pragma unroll
+      for (int c = 0; c < C; ++c) o[c] *= a;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        if (first + k * WARPS > g1) break;
+        const float w = exp2f(st[k].x - ref);
+        l += st[k].y * w;
+#pragma unroll
+        for (int c = 0; c < C; ++c) o[c] += v[k][c] * w;
+      }
     }
     if constexpr (WARPS > 1) {
 #pragma unroll
       for (int c = 0; c < C; ++c) sums[warp][lane * C + c] = o[c];
-      if (lane == 0) parts[warp] = l;
+      if (lane == 0) parts[warp] = make_float2(top, l);
       __syncthreads();
       if (part == 0) {
 #pragma unroll
-        for (int k = 1; k < WARPS; ++k) {
-          l += parts[warp + k];
+        for (int k = 1; k < WARPS; ++k) top = fmaxf(top, parts[warp + k].x);
+        const float ref = top == -INFINITY ? 0.f : top;
+        l = 0.f;
 #pragma unroll
-          for (int c = 0; c < C; ++c) o[c] += sums[warp + k][lane * C + c];
+        for (int c = 0; c < C; ++c) o[c] = 0.f;
+#pragma unroll
+        for (int k = 0; k < WARPS; ++k) {
+          const float w = exp2f(parts[warp + k].x - ref);
+          l += parts[warp + k].y * w;
+#pragma unroll
+          for (int c = 0; c < C; ++c) o[c] += sums[warp + k][lane * C + c] * w;
         }
       }
       __syncthreads();
