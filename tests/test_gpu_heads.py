@@ -119,7 +119,7 @@ def run_case(b, n, hq, hk, d, rotary, dtype, weights=None, wdtype=None, fused=Tr
 
 @pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize('layout', ['interleaved', 'half'])
-@pytest.mark.parametrize('d, r', [(64, 64), (64, 32), (128, 128), (128, 48), (80, 40), (256, 256), (256, 2), (96, 6), (34, 34), (36, 20), (2, 2), (250, 126)])
+@pytest.mark.parametrize('d, r', [(64, 64), (64, 32), (128, 128), (128, 48), (80, 40), (256, 256), (256, 2), (96, 6), (34, 34), (36, 20), (2, 2), (250, 126), (128, 20), (80, 20)])
 @pytest.mark.parametrize('weights', [None, 'shared', 'heads'])
 def test_layouts_and_parts(dtype, layout, d, r, weights):
     run_case(2, 13, 6, 2, d, RotaryFrequencies(d, r, layout=layout), dtype, weights)
@@ -360,3 +360,40 @@ def test_refusals_on_the_device():
     for call, match in cases:
         with pytest.raises(L.NsaError, match=match):
             call()
+
+
+def test_two_streams_at_once():
+    rotary = RotaryFrequencies(128, layout='half')
+    w = [(1 + randn((128,), i, torch.bfloat16, 0.2)).requires_grad_() for i in (1, 2)]
+    xs = [randn((2, h, n, 128), 3 + n, torch.bfloat16) for h, n in ((8, 700), (4, 900))]
+
+    def step(x):
+        leaf = x.detach().requires_grad_()
+        y, z = norm_rotate_heads(leaf, leaf, *w, rotary)
+        return torch.autograd.grad((y, z), (leaf, *w), (y.detach(), z.detach()))
+    expected = [step(x) for x in xs]
+    streams = [torch.cuda.Stream() for _ in xs]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(10):
+        for i, x in enumerate(xs):
+            with torch.cuda.stream(streams[i]):
+                got[i].append(step(x))
+    torch.cuda.synchronize()
+    for g, e in zip(got, expected):
+        for grads in g:
+            for a, b in zip(grads, e):
+                assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize('layout', ['interleaved', 'half'])
+def test_weights_on_narrow_boundaries(layout):
+    """fp32 weights beside bf16 rows, and bf16 ones, as views into a flat buffer of parameters."""
+    rotary, x = RotaryFrequencies(64, layout=layout), randn((1, 3, 6, 64), 1, torch.bfloat16)
+    angle = angles(rotary, torch.arange(6, device=DEV))
+    for dtype in (torch.float32, torch.bfloat16):
+        flat = 1 + randn((64 * 3 + 8,), 2, dtype, 0.3)
+        for shift in (0, 1, 2, 4):
+            for w in (flat[shift:shift + 64], flat[shift:shift + 192].view(3, 64)):
+                y, _ = norm_rotate_heads(x, None, w, None, rotary)
+                check_forward(x, w, y, rotary, angle, torch.finfo(torch.float32).eps, f'{dtype} {shift}')
