@@ -153,6 +153,12 @@ __device__ __forceinline__ const T* row_of(const RowView& r, int b, int h, int64
 
 // ---- any type and alignment, on the CUDA cores -------------------------------------------
 
+// fp32, and bf16 rows that TMA cannot fetch.  256 threads share a tile of 8, 32 or 64 rows: scores of a block into shared memory, softmax
+// by 32, 8 or 4 lanes a row, values times weights in registers.  Bound by shared memory and issue: with 64 rows a thread has 4 rows x 2
+// keys, then 4 x 8 columns, eight and nine 16-byte reads for 32 and 128 fused multiplications of a step.  fp32 rows arrive a block ahead.
+// 4 x 64 tokens over 4096 rows, 64 / 8 heads of 128: 977 us, 30 TFLOP/s (tiles of 32 rows, loads in turn, columns read one by one: 1712);
+// 16 x one token over 8192 rows, 32 / 4 heads of 128: 126 us, 3.2 TB/s (two rows x one key a thread: 167).
+
 namespace tree_simt {
 constexpr int kThreads = 256;
 template <int DP, int RT>
@@ -160,11 +166,12 @@ struct Shape {
   static constexpr int kKeys = RT == 8 ? 64 : 32;           // of a block; two are in shared memory
   static constexpr int kRow = DP + 4;                       // padded: four neighbouring rows on different banks
   static constexpr int kScore = kKeys + 4;
-  static constexpr int TX = RT == 8 ? 64 : 16, TY = kThreads / TX;
+  static constexpr int TX = RT == 8 ? 32 : 16, TY = kThreads / TX;
   static constexpr int KPT = kKeys / TX, RPT = RT / TY;     // keys and rows of a thread
+  static constexpr int kPlanes = RT == 8 ? 4 : 1;           // eight rows: scores by quarters of the features
   static constexpr int CPT = DP / TX;                       // output columns of a thread, VC neighbours every VC TX
   static constexpr int VC = CPT < 4 ? CPT : 4;
-  static constexpr int kFloats = RT * kRow + 4 * kKeys * kRow + RT * kScore + 3 * RT;
+  static constexpr int kFloats = RT * kRow + 4 * kKeys * kRow + kPlanes * RT * kScore + 3 * RT;
   static constexpr int kPerSM = kFloats * 4 <= 113 * 1024 ? 2 : 1;          // CTAs
 };
 }  // namespace tree_simt
@@ -180,7 +187,7 @@ __global__ void __launch_bounds__(tree_simt::kThreads, tree_simt::Shape<DP, RT>:
   float* const qs = tree_smem;
   float* const tiles = qs + RT * S::kRow;               // K and V of two blocks
   float* const ss = tiles + 4 * kKeys * S::kRow;
-  float* const row_m = ss + RT * S::kScore;
+  float* const row_m = ss + S::kPlanes * RT * S::kScore;
   float* const row_l = row_m + RT;
   float* const row_a = row_l + RT;
   __shared__ int odd_values;       // a drafted value of this unit is not finite
@@ -254,9 +261,12 @@ __global__ void __launch_bounds__(tree_simt::kThreads, tree_simt::Shape<DP, RT>:
       qs[r * S::kRow + c] = row < rows && c < P.d ? Elem<T>::to_float(row_of<T>(P.q, at.b, h * P.G + g, t)[c]) : 0.f;
     }
     if (tid < RT) { row_m[tid] = -INFINITY; row_l[tid] = 0.f; }
-    float o[S::RPT][S::CPT];
+    // Eight rows: a thread takes all of them, for one key and a quarter of the features, then for an eighth of the keys (its warp's) and
+    // its columns, so that K and V are read from shared memory once; the warps' sums are added at the unit's end.
+    constexpr int ROWS = RT == 8 ? 8 : S::RPT;
+    float o[ROWS][S::CPT];
 #pragma unroll
-    for (int r = 0; r < S::RPT; ++r)
+    for (int r = 0; r < ROWS; ++r)
 #pragma unroll
       for (int c = 0; c < S::CPT; ++c) o[r][c] = 0.f;
 
@@ -298,33 +308,51 @@ __global__ void __launch_bounds__(tree_simt::kThreads, tree_simt::Shape<DP, RT>:
       }
       __syncthreads();
 
-      // scores: keys tx + TX k, rows ty RPT + r
-      float s[S::RPT][S::KPT];
+      if constexpr (RT == 8) {
+        const int key = tid & 63, part = tid >> 6;
+        float d[8];
 #pragma unroll
-      for (int r = 0; r < S::RPT; ++r)
-#pragma unroll
-        for (int k = 0; k < S::KPT; ++k) s[r][k] = 0.f;
+        for (int r = 0; r < 8; ++r) d[r] = 0.f;
 #pragma unroll 4
-      for (int c = 0; c < DP; c += 4) {
-        float4 kv[S::KPT], qv[S::RPT];
+        for (int c = part * (DP / 4); c < (part + 1) * (DP / 4); c += 4) {
+          const float4 kv = *reinterpret_cast<const float4*>(ks + key * S::kRow + c);
 #pragma unroll
-        for (int k = 0; k < S::KPT; ++k) kv[k] = *reinterpret_cast<const float4*>(ks + (tx + S::TX * k) * S::kRow + c);
+          for (int r = 0; r < 8; ++r) {
+            const float4 qv = *reinterpret_cast<const float4*>(qs + r * S::kRow + c);
+            d[r] += qv.x * kv.x + qv.y * kv.y + qv.z * kv.z + qv.w * kv.w;
+          }
+        }
 #pragma unroll
-        for (int r = 0; r < S::RPT; ++r) qv[r] = *reinterpret_cast<const float4*>(qs + (ty * S::RPT + r) * S::kRow + c);
+        for (int r = 0; r < 8; ++r) ss[(part * 8 + r) * S::kScore + key] = d[r];
+      } else {
+        // scores: keys tx + TX k, rows ty RPT + r
+        float s[S::RPT][S::KPT];
 #pragma unroll
         for (int r = 0; r < S::RPT; ++r)
 #pragma unroll
-          for (int k = 0; k < S::KPT; ++k)
-            s[r][k] += qv[r].x * kv[k].x + qv[r].y * kv[k].y + qv[r].z * kv[k].z + qv[r].w * kv[k].w;
-      }
+          for (int k = 0; k < S::KPT; ++k) s[r][k] = 0.f;
+#pragma unroll 4
+        for (int c = 0; c < DP; c += 4) {
+          float4 kv[S::KPT], qv[S::RPT];
 #pragma unroll
-      for (int r = 0; r < S::RPT; ++r)
+          for (int k = 0; k < S::KPT; ++k) kv[k] = *reinterpret_cast<const float4*>(ks + (tx + S::TX * k) * S::kRow + c);
 #pragma unroll
-        for (int k = 0; k < S::KPT; ++k) {
-          const int key = tx + S::TX * k, row = row0 + ty * S::RPT + r;
-          const bool ok = key < n && row < rows && (!draft || sees(P, at.b, row / P.G, first + key));
-          ss[(ty * S::RPT + r) * S::kScore + key] = ok ? s[r][k] * scale2 : -INFINITY;
+          for (int r = 0; r < S::RPT; ++r) qv[r] = *reinterpret_cast<const float4*>(qs + (ty * S::RPT + r) * S::kRow + c);
+#pragma unroll
+          for (int r = 0; r < S::RPT; ++r)
+#pragma unroll
+            for (int k = 0; k < S::KPT; ++k)
+              s[r][k] += qv[r].x * kv[k].x + qv[r].y * kv[k].y + qv[r].z * kv[k].z + qv[r].w * kv[k].w;
         }
+#pragma unroll
+        for (int r = 0; r < S::RPT; ++r)
+#pragma unroll
+          for (int k = 0; k < S::KPT; ++k) {
+            const int key = tx + S::TX * k, row = row0 + ty * S::RPT + r;
+            const bool ok = key < n && row < rows && (!draft || sees(P, at.b, row / P.G, first + key));
+            ss[(ty * S::RPT + r) * S::kScore + key] = ok ? s[r][k] * scale2 : -INFINITY;
+          }
+      }
       __syncthreads();
 
       // softmax: kThreads / RT lanes share a row
@@ -333,7 +361,16 @@ __global__ void __launch_bounds__(tree_simt::kThreads, tree_simt::Shape<DP, RT>:
         const int r = tid / L, l = tid % L;
         float x[E], m = -INFINITY;
 #pragma unroll
-        for (int i = 0; i < E; ++i) { x[i] = ss[r * S::kScore + l + i * L]; m = fmaxf(m, x[i]); }
+        for (int i = 0; i < E; ++i) {
+          x[i] = ss[r * S::kScore + l + i * L];
+          if constexpr (RT == 8) {
+#pragma unroll
+            for (int k = 1; k < 4; ++k) x[i] += ss[(k * 8 + r) * S::kScore + l + i * L];
+            const int key = l + i * L;
+            x[i] = key < n && r < rows && (!draft || sees(P, at.b, r / P.G, first + key)) ? x[i] * scale2 : -INFINITY;
+          }
+          m = fmaxf(m, x[i]);
+        }
 #pragma unroll
         for (int off = L / 2; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor_sync(kFullMask, m, off));
         const float m_old = row_m[r], m_new = fmaxf(m_old, m), ref = m_new == -INFINITY ? 0.f : m_new;
@@ -357,17 +394,18 @@ __global__ void __launch_bounds__(tree_simt::kThreads, tree_simt::Shape<DP, RT>:
       __syncthreads();
 
       // output columns: column(c)
+      const int first_row = RT == 8 ? 0 : ty * S::RPT, first_key = RT == 8 ? ty * 8 : 0, last_key = RT == 8 ? first_key + 8 : kKeys;
 #pragma unroll
-      for (int r = 0; r < S::RPT; ++r) {
-        const float a = row_a[ty * S::RPT + r];
+      for (int r = 0; r < ROWS; ++r) {
+        const float a = row_a[first_row + r];
 #pragma unroll
         for (int c = 0; c < S::CPT; ++c) o[r][c] *= a;
       }
 #pragma unroll 2
-      for (int k = 0; k < kKeys; k += 4) {
-        float4 p[S::RPT];
+      for (int k = first_key; k < last_key; k += 4) {
+        float4 p[ROWS];
 #pragma unroll
-        for (int r = 0; r < S::RPT; ++r) p[r] = *reinterpret_cast<const float4*>(ss + (ty * S::RPT + r) * S::kScore + k);
+        for (int r = 0; r < ROWS; ++r) p[r] = *reinterpret_cast<const float4*>(ss + (first_row + r) * S::kScore + k);
 #pragma unroll
         for (int kk = 0; kk < 4; ++kk) {
           float v[S::CPT];
@@ -385,12 +423,26 @@ __global__ void __launch_bounds__(tree_simt::kThreads, tree_simt::Shape<DP, RT>:
             }
           }
 #pragma unroll
-          for (int r = 0; r < S::RPT; ++r) {
+          for (int r = 0; r < ROWS; ++r) {
             const float w = kk == 0 ? p[r].x : kk == 1 ? p[r].y : kk == 2 ? p[r].z : p[r].w;
 #pragma unroll
             for (int c = 0; c < S::CPT; ++c) o[r][c] += w * v[c];
           }
         }
+      }
+    }
+    if constexpr (RT == 8) {
+      __syncthreads();           // the tiles have been read
+#pragma unroll
+      for (int r = 0; r < 8; ++r)
+#pragma unroll
+        for (int c = 0; c < S::CPT; ++c) tiles[(ty * 8 + r) * DP + column(c)] = o[r][c];
+      __syncthreads();
+#pragma unroll
+      for (int c = 0; c < S::CPT; ++c) {      // warp ty has row ty now
+        o[0][c] = 0.f;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) o[0][c] += tiles[(k * 8 + ty) * DP + column(c)];
       }
     }
 
@@ -447,11 +499,13 @@ __global__ void __launch_bounds__(tree_simt::kThreads, tree_simt::Shape<DP, RT>:
 //   mending warp    clears the rows of a V block that lie behind the sequence, and drafted values that are not finite
 //   MMA warp(s)     S = Q K^T, then O += P V with P from tensor memory; one per stream
 //   softmax warps   S from tensor memory, maximum, exponentials, P back as bf16.  A warp reaches 32 lanes of tensor memory, 32 rows.
-//                   One stream: two threads per row, half of a block's keys each, which exchange maxima (one token over 4096 rows
-//                   10.1 us, with one thread 11.4).  Two streams: one thread (64 tokens over 65536 rows 502 us, with two 588).  P is rounded (2^-9 on average a weight, as any bf16 tensor of
+//                   One stream: two threads per row, half of a block's keys each, which exchange maxima.  Two streams: one thread (64
+//                   tokens over 65536 rows, a block of 64 keys and two tiles: 1790 cycles, with two threads 2000).  P is rounded (2^-9 on average a weight, as any bf16 tensor of
 //                   weights would be); the sum adds the exponentials as they are.
 // The accumulator O stays in tensor memory.  It is rescaled lazily: a row keeps its reference maximum until a block exceeds it by
 // more than 2^8.
+// What bounds it: the exponentials (16 a cycle and SM) and what else a warp does for a value beside them; then power.  64 tokens over 65536
+// rows, 64 / 8 heads of 128: 388 us, 1190 TFLOP/s, in bursts of 30 passes, 460 us back to back (1.5 GHz at 990 W).
 // STREAMS.  Above 128 rows two tiles share the K and V blocks; the softmax of one runs under the products of the other.  Blocks of 64
 // keys, so that tensor memory holds two S buffers of either beside both O: with blocks of 128 and one buffer, S of the next block
 // waited for the products of this one, which waited for its softmax (3800 cycles a block and pair of tiles, 2050 of them products).
