@@ -610,6 +610,8 @@ static int launch_heads_w(HeadsParams& P, cudaStream_t stream) {
   const int rc = heads_grid(P, partials, partials && WEIGHTS == heads::kPerHead, heads::kThreads >> P.lane_shift);
   if (rc != NSA_OK) return rc;
   const unsigned grid = (unsigned)(P.slots[0] * P.blocks[0] + P.slots[1] * P.blocks[1]);
+  const int rows = P.weight_per_head ? P.part[0].heads + P.part[1].heads : (P.part[0].heads > 0) + (P.part[1].heads > 0);
+  if (partials && rows > 65535) return fail(NSA_ERR_SHAPE, "heads: more than 65535 weight rows");
   const bool full = W * (int)sizeof(T) == 16 && P.d == (2 * W << P.lane_shift);      // the usual heads, in the widest vectors
   constexpr bool wide = W * sizeof(T) == 16;
   if (full && P.half) heads_kernel<T, W, UPL, true, WEIGHTS, BWD, wide><<<grid, heads::kThreads, 0, stream>>>(P);
@@ -618,8 +620,6 @@ static int launch_heads_w(HeadsParams& P, cudaStream_t stream) {
   else heads_kernel<T, W, UPL, false, WEIGHTS, BWD, false><<<grid, heads::kThreads, 0, stream>>>(P);
   cudaError_t err = cudaGetLastError();
   if (partials && err == cudaSuccess) {
-    const int rows = P.weight_per_head ? P.part[0].heads + P.part[1].heads : (P.part[0].heads > 0) + (P.part[1].heads > 0);
-    if (rows > 65535) return fail(NSA_ERR_SHAPE, "heads: more than 65535 weight rows");
     cudaLaunchConfig_t config = {};      // starts while the last blocks of the kernel before it are at work
     config.gridDim = dim3((unsigned)(P.d + 7) / 8, (unsigned)rows);
     config.blockDim = dim3(1024);
