@@ -27,12 +27,6 @@ __device__ __forceinline__ int length_of(const TreeParams& P, int b) {
   return max(0, min(n, P.capacity));
 }
 
-__device__ __forceinline__ int warp_add(int v) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(kFullMask, v, o);
-  return v;
-}
-
 // Key blocks of one KV head of a sequence
 template <int KB>
 __device__ __forceinline__ int cache_blocks(const TreeParams& P, int b) { return (length_of(P, b) + KB - 1) / KB; }
@@ -667,6 +661,7 @@ __device__ __forceinline__ void mend_blocks(const TreeParams& P, tree::Walk<KK>&
         fence_proxy_async_smem();
         odd = __any_sync(kFullMask, odd);
       }
+      __syncwarp();          // what all lanes wrote lies before the arrival
       if (lane == 0) {
         if (j == walk.j1 - 1) odd_values[seq & 15] = odd;
         mbar_arrive(smem_u32(&bars.ready[u % kAhead]));
@@ -1428,7 +1423,7 @@ __global__ void __launch_bounds__(256) tree_merge_kernel(const TreeParams P) {
 
 struct TreePlan {
   bool tensor_cores;
-  int DP, RT, KB, streams;   // padded dim_head, rows of a tile, keys of a block
+  int DP, RT, KB;            // padded dim_head, rows of a tile, keys of a block
   int tiles, groups;
   int64_t partial_bytes, bytes;
 };
