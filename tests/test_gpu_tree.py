@@ -295,6 +295,17 @@ def test_streams_graphs_and_repeats(dtype):
     ops.check_device_status()
 
 
+def test_gradients_are_refused_not_dropped():
+    args = problem(1, 3, 4, 2, 64, 10, torch.bfloat16)
+    expected = tree_attend(*args[:3], None, *args[3:])
+    for i in range(5):
+        given = [x.clone().requires_grad_(j == i) for j, x in enumerate(args)]
+        with pytest.raises(L.NsaError, match='no gradient'):
+            tree_attend(*given[:3], None, *given[3:])
+        with torch.no_grad():
+            assert torch.equal(tree_attend(*given[:3], None, *given[3:]), expected)
+
+
 def test_refusals_on_the_device():
     q, kc, vc, k, v = problem(2, 3, 4, 2, 64, 10, torch.float32)
     ok = torch.zeros(2, dtype=torch.int32, device=DEV)
