@@ -1,5 +1,6 @@
 // Rotation of queries and keys by their positions, with or without their norm: the call, and the autograd node around it.
 
+#include <ATen/MemoryOverlap.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/saved_variable.h>
@@ -59,6 +60,19 @@ nsa_heads_args head_args(const Rotation& r, const Tensor& like) {
   return a;
 }
 
+// A thread reads its part of a row before it writes it, so an output may be the tensor that it belongs to, and none of the others
+void check_output(const Tensor& out, const Tensor& own, const Tensor& other, const Tensor& other_out) {
+  using at::MemOverlapStatus;
+  auto shared = [&](const Tensor& t) {
+    const MemOverlapStatus s = at::get_overlap_status(out, t);
+    return s == MemOverlapStatus::Full || s == MemOverlapStatus::Partial;
+  };
+  require(at::has_internal_overlap(out) != at::MemOverlap::Yes, "an output must not be broadcast");
+  require(at::get_overlap_status(out, own) != MemOverlapStatus::Partial, "an output may be the tensor itself, but must not overlap it otherwise");
+  require((!other.defined() || !shared(other)) && (!other_out.defined() || !shared(other_out)), "an output of one of the tensors must not overlap the other's");
+  require(!at::GradMode::is_enabled() || !out.requires_grad(), "an output that wants gradients itself cannot be given");
+}
+
 // Shapes that do not fit the C structs' 32 bits
 void check_sizes(const Tensor& t) {
   for (int64_t s : t.sizes()) require(s <= 0x7fffffff, "a size is above 2^31");
@@ -89,12 +103,14 @@ struct Gradients {
 struct RotatedHeadsBackward : torch::autograd::Node {
   Rotation r;
   torch::autograd::SavedVariable x[2], w[2];     // with norm
+  torch::autograd::SavedVariable positions;      // kept as a saved tensor, so that one overwritten before the backward pass is refused
   // what the gradients look like (without norm nothing of the inputs is kept)
   at::TensorOptions options;
   std::vector<int64_t> sizes[2], strides[2];
+  bool by_positions = false;
 
   void release_variables() override {
-    for (auto* t : {&x[0], &x[1], &w[0], &w[1]}) t->reset_data();
+    for (auto* t : {&x[0], &x[1], &w[0], &w[1], &positions}) t->reset_data();
   }
 
   torch::autograd::variable_list apply(torch::autograd::variable_list&& grads) override {
@@ -109,7 +125,9 @@ struct RotatedHeadsBackward : torch::autograd::Node {
         xs[i] = x[i].unpack(getptr());
         ws[i] = w[i].unpack(getptr());
       }
-      Gradients g = heads_backward(xs, ws, dy);
+      Rotation turn = r;
+      if (by_positions) turn.positions = positions.unpack(getptr());
+      Gradients g = heads_backward(turn, xs, ws, dy);
       for (int i = 0; i < 2; ++i) {
         if (task_should_compute_output(i)) out[i] = g.dx[i];
         if (r.norm && task_should_compute_output(2 + i)) out[2 + i] = g.dw[i];
@@ -126,11 +144,11 @@ struct RotatedHeadsBackward : torch::autograd::Node {
     return out;
   }
 
-  Gradients heads_backward(const Tensor* x, const Tensor* w, const Tensor* dy) const;
+  Gradients heads_backward(const Rotation& r, const Tensor* x, const Tensor* w, const Tensor* dy) const;
 };
 
 // A tensor whose result gets no gradient has none itself
-Gradients RotatedHeadsBackward::heads_backward(const Tensor* x, const Tensor* w, const Tensor* dy) const {
+Gradients RotatedHeadsBackward::heads_backward(const Rotation& r, const Tensor* x, const Tensor* w, const Tensor* dy) const {
   const c10::cuda::CUDAGuard guard(options.device());
   Gradients g;
   Tensor rows[2];
@@ -195,6 +213,8 @@ static std::vector<OptTensor> rotate_heads(Tensor q, OptTensor k_, OptTensor wq,
                   (x[i].size(3) == 1 || given[i].stride(3) == 1),
               "an output must have the tensor's device, type and shape, and a contiguous last axis");
   }
+  for (int i = 0; i < 2; ++i)
+    if (given[i].defined()) check_output(given[i], x[i], x[1 - i], given[1 - i]);
   wanted = wanted && at::GradMode::is_enabled();
   require(!wanted || (!given[0].defined() && !given[1].defined()), "outputs cannot be given where gradients are wanted");
   if (positions.has_value() && positions->defined()) {
@@ -227,6 +247,8 @@ static std::vector<OptTensor> rotate_heads(Tensor q, OptTensor k_, OptTensor wq,
       }
     }
     check(nsa_heads_fwd(&a, stream_of(q)));
+    for (const Tensor& t : given)        // as any write in place: whoever saved these for a backward pass learns of it
+      if (t.defined() && !t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
   }
   if (wanted) {
     using torch::autograd::SavedVariable;
@@ -234,6 +256,9 @@ static std::vector<OptTensor> rotate_heads(Tensor q, OptTensor k_, OptTensor wq,
     auto edge = [](const Tensor& t) { return t.defined() ? torch::autograd::impl::gradient_edge(t) : torch::autograd::Edge(); };
     node->set_next_edges({edge(x[0]), edge(x[1]), edge(w[0]), edge(w[1])});
     node->r = r;
+    node->r.positions = Tensor();
+    node->by_positions = r.positions.defined();
+    if (node->by_positions) node->positions = SavedVariable(r.positions.is_inference() ? r.positions.clone() : r.positions, false);
     node->options = q.options();
     for (int i = 0; i < 2; ++i) {
       if (!x[i].defined()) continue;

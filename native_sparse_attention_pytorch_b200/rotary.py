@@ -182,6 +182,6 @@ def rotate_heads(q, k, rotary, positions=None, offset=0, out=None):
     """Queries and keys rotated by their positions, in one launch: q [b, q_heads, n, d], k [b, kv_heads, n, d] (or None) ->
     the same shapes, contiguous; fp32 arithmetic, rounded once.  float32 or bfloat16, any strides with a contiguous last
     axis.  `positions`: int64 or int32, [n] or [b, n] (default 0 .. n-1), `offset` is added to them.  `out`: a pair of
-    tensors to write instead (rows of a cache, or q and k themselves), where no gradient is wanted.  Differentiable in q and
-    k; gradients keep the memory order of their inputs."""
+    tensors to write instead (rows of a cache, or q and k themselves, each in its own place), where no gradient is wanted.
+    Differentiable in q and k; gradients keep the memory order of their inputs."""
     return _rotate(q, k, None, None, rotary, positions, offset, False, 0.0, out)

@@ -362,6 +362,53 @@ def test_refusals_on_the_device():
             call()
 
 
+def test_outputs_that_overlap_are_refused():
+    rotary, w = RotaryFrequencies(64), torch.ones(64, device=DEV)
+    q, k = randn((2, 3, 5, 64), 1), randn((2, 3, 5, 64), 2)
+    flat = randn((2 * 3 * 5 * 64 + 64,), 3)
+    cases = [
+        (lambda: rotate_heads(q, k, rotary, out=(k, None)), "overlap the other"),
+        (lambda: rotate_heads(q, k, rotary, out=(k, q)), "overlap the other"),
+        (lambda: rotate_heads(q, k, rotary, out=(flat[64:].view_as(q), flat[:-64].view_as(q))), "overlap the other"),
+        (lambda: rotate_heads(flat[64:].view_as(q), None, rotary, out=(flat[:-64].view_as(q), None)), 'must not overlap it'),
+        (lambda: rotate_heads(q, None, rotary, out=(q[:, :1].expand(2, 3, 5, 64), None)), 'broadcast'),
+        (lambda: norm_rotate_heads(q, None, w, None, rotary, out=(flat[64:].view_as(q).requires_grad_(), None)), 'wants gradients'),
+    ]
+    before = q.clone(), k.clone(), flat.clone()
+    for call, match in cases:
+        with pytest.raises(L.NsaError, match=match):
+            call()
+    flat = flat.detach()
+    assert all(torch.equal(a, b) for a, b in zip(before, (q, k, flat)))
+    qkv = randn((2, 5, 9, 64), 4).transpose(1, 2)          # one projection's heads, side by side, each in its own place
+    a, b = qkv[:, :6], qkv[:, 6:8]
+    y, z = rotate_heads(a.contiguous(), b.contiguous(), rotary)
+    rotate_heads(a, b, rotary, out=(a, b))
+    assert torch.equal(a, y) and torch.equal(b, z)
+
+
+def test_what_a_backward_pass_needs_is_not_overwritten_unnoticed():
+    rotary = RotaryFrequencies(64)
+    x, at = randn((1, 2, 3, 64), 1).requires_grad_(), torch.tensor([4, 5, 9], device=DEV)
+    y, _ = rotate_heads(x, None, rotary, at)
+    at.add_(1)                                               # the positions of the next step, in the same tensor
+    with pytest.raises(RuntimeError, match='modified by an inplace operation'):
+        y.sum().backward()
+    e = x.exp()                                              # its backward pass needs its result
+    with torch.no_grad():
+        rotate_heads(e, None, rotary, out=(e, None))
+    with pytest.raises(RuntimeError, match='modified by an inplace operation'):
+        e.sum().backward()
+    with torch.inference_mode():
+        then = torch.tensor([4, 5, 9], device=DEV)
+        t = torch.zeros(1, 2, 3, 64, device=DEV)
+        rotate_heads(t, None, rotary, then, out=(t, None))
+    y, _ = rotate_heads(x, None, rotary, then)
+    dx, = torch.autograd.grad(y, x, torch.ones_like(y))
+    ref = turned(torch.ones_like(y), rotary, angles(rotary, torch.tensor([4, 5, 9], device=DEV)), inverse=True)
+    assert (dx.double() - ref).abs().max() <= 64 * U
+
+
 def test_two_streams_at_once():
     rotary = RotaryFrequencies(128, layout='half')
     w = [(1 + randn((128,), i, torch.bfloat16, 0.2)).requires_grad_() for i in (1, 2)]
