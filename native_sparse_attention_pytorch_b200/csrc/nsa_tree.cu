@@ -619,7 +619,10 @@ __device__ __forceinline__ void fetch_blocks(const TreeParams& P, const TreeAxes
     mbar_wait_drain(smem_u32(&bars.full[(i - back) % SLOTS]), ((i - back) / SLOTS) & 1);
 }
 
-// The role of the mending warp: rows of a V block behind the sequence are cleared, as are drafted values that are not finite
+// The role of the mending warp: rows of a V block behind the sequence are cleared, as are drafted values that are not finite.  It asks
+// about every block in turn, and a barrier is asked by the parity of its phase: a slot must not be filled again before this warp has
+// seen it full (the phase it asks for would be over, and the next one of that parity waits for this warp), and it must not ask about a
+// phase before the one in front of it is over (a slot may hold K and V in turn).  So it waits for K as well, and gives slots back.
 template <int D, int KK, int SLOTS>
 __device__ __forceinline__ void mend_blocks(const TreeParams& P, tree::Walk<KK>& walk, uint32_t ring, tree_tc::Bars& bars, volatile int* odd_values, int lane,
                                             volatile int* abort_flag) {
@@ -633,8 +636,8 @@ __device__ __forceinline__ void mend_blocks(const TreeParams& P, tree::Walk<KK>&
     for (int j = walk.j0; j < walk.j1; ++j, ++u) {
       const uint32_t slot = (2 * u + 1) % SLOTS, round = (2 * u + 1) / SLOTS;
       const uint32_t at = ring + slot * kTile;
-      // the K block as well: a slot that holds K and V in turn must not be asked about a phase before the one before it is over
       mbar_wait_warp(smem_u32(&bars.full[2 * u % SLOTS]), (2 * u / SLOTS) & 1, abort_flag);
+      if (lane == 0) mbar_arrive(smem_u32(&bars.free[2 * u % SLOTS]));
       mbar_wait_warp(smem_u32(&bars.full[slot]), round & 1, abort_flag);
       const bool draft = j >= walk.cached;
       const int n = min(KK, (draft ? P.tokens - (j - walk.cached) * KK : walk.length - j * KK));
@@ -665,6 +668,7 @@ __device__ __forceinline__ void mend_blocks(const TreeParams& P, tree::Walk<KK>&
       if (lane == 0) {
         if (j == walk.j1 - 1) odd_values[seq & 15] = odd;
         mbar_arrive(smem_u32(&bars.ready[u % kAhead]));
+        mbar_arrive(smem_u32(&bars.free[slot]));
       }
       __syncwarp();
     }
@@ -707,7 +711,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmKc, const __grid_constant__
     abort_flag = sQ0 & 1023u ? 1 : 0;                   // the tiles would be mis-swizzled: report instead of computing
     for (int i = 0; i < kSlots; ++i) {
       mbar_init(smem_u32(&bars.full[i]), 1);
-      mbar_init(smem_u32(&bars.free[i]), streams);
+      mbar_init(smem_u32(&bars.free[i]), streams + 1);      // the products of each stream, the mending warp
     }
     for (int i = 0; i < kAhead; ++i) mbar_init(smem_u32(&bars.ready[i]), 1);
     for (int s = 0; s < streams; ++s) {
@@ -1051,7 +1055,7 @@ tree_few_kernel(const __grid_constant__ CUtensorMap tmKc, const __grid_constant_
     abort_flag = sRing & 1023u ? 1 : 0;                  // the tiles would be mis-swizzled: report instead of computing
     for (int i = 0; i < kSlots; ++i) {
       mbar_init(smem_u32(&bars.full[i]), 1);
-      mbar_init(smem_u32(&bars.free[i]), 1);
+      mbar_init(smem_u32(&bars.free[i]), 2);                // the products, the mending warp
     }
     for (int i = 0; i < kAhead; ++i) mbar_init(smem_u32(&bars.ready[i]), 1);
     mbar_init(smem_u32(&bars.q_full[0]), kSoft);
