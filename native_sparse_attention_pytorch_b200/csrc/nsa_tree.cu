@@ -984,8 +984,9 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmKc, const __grid_constant__
 // multiple of 16): S^T = K Q^T [128 keys x N], O^T += V^T P^T [dim_head x N].  A thread has a key (two or four threads share one, eight or
 // sixteen columns each) and exponentials for the rows there are; P^T goes through shared memory, K-major as the products want it.
 //   * The reference maxima are one per column, the same for all threads, in shared memory.  While no logit exceeds its column's by
-//     more than 2^8 (one vote of all softmax warps a block) nothing is reduced over the keys; else, and for the first block of a unit
-//     and those of the drafted rows, the maxima are taken, O^T and the sums rescaled.
+//     more than 2^8 (one vote of all softmax warps a block) nothing is reduced over the keys; else, for the first block of a unit, for
+//     those behind it while a column has seen nothing but -inf, and for those of the drafted rows, the maxima are taken, O^T and the
+//     sums rescaled.
 //   * Sums stay with the threads, a key each, until a unit ends.
 //   * The transposed accumulator leaves whole rows of the output side by side.
 // Against the tile with rows as rows and copies of them over the keys, calls back to back: one token over 4096 rows 12.3 -> 11.6 us, 32
@@ -1042,8 +1043,9 @@ tree_few_kernel(const __grid_constant__ CUtensorMap tmKc, const __grid_constant_
   __shared__ uint32_t tmem_slot;
   __shared__ __align__(8) Bars bars;
   __shared__ volatile int odd_values[16];               // by unit: a drafted value is not finite
-  // by column: the reference maximum (base 2; -inf: nothing seen yet), what is added to the logits (0 for that; -inf for a column
-  // without a row, whose weights are then zero), the factor of a rescaling, at a unit's end the sum
+  // by column: the reference maximum (base 2; -inf: nothing seen yet), what is added to the logits (0 for that: they are all -inf, and
+  // the next block's maxima are taken; -inf for a column without a row, whose weights are then zero), the factor of a rescaling, at a
+  // unit's end the sum
   __shared__ __align__(16) float ref[N], off[N], factor[N], sums[N];
   __shared__ float found[4][N];                         // maxima, and sums at a unit's end, of the quarters of the keys
 
@@ -1136,6 +1138,7 @@ tree_few_kernel(const __grid_constant__ CUtensorMap tmKc, const __grid_constant_
       float l[NT];
 #pragma unroll
       for (int c = 0; c < NT; ++c) l[c] = 0.f;
+      bool open = true;         // a column has no reference yet (all its logits were -inf): the same for all softmax warps
       for (int j = walk.j0; j < walk.j1; ++j, ++u) {
         const uint32_t buf = u & 1, phase = (u >> 1) & 1;
         const bool draft = j >= walk.cached;
@@ -1164,7 +1167,7 @@ tree_few_kernel(const __grid_constant__ CUtensorMap tmKc, const __grid_constant_
             unpack2(fma2(pack2(x[c + 2], x[c + 3]), scale, pack2(o.z, o.w)), y[c + 2], y[c + 3]);
           }
         };
-        bool renew = j == walk.j0 || draft;
+        bool renew = open || draft;
         if (!renew) {
           shift();
           renew = soft_any(max_row<NT>(y) > 8.f);
@@ -1184,7 +1187,7 @@ tree_few_kernel(const __grid_constant__ CUtensorMap tmKc, const __grid_constant_
           } else if (tid < N) {
             factor[tid] = 1.f;
           }
-          soft_sync();
+          open = soft_any(tid < here && ref[tid] == -INFINITY);
 #pragma unroll
           for (int c = 0; c < NT; ++c) l[c] *= factor[col0 + c];
           if (j > walk.j0) {
