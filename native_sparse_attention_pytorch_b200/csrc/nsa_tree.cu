@@ -91,6 +91,12 @@ __device__ __forceinline__ int group_of(int64_t total, int64_t x, int groups) {
   return (uint64_t)(y | total) >> 32 ? (int)(y / total) : (int)((uint32_t)y / (uint32_t)total);
 }
 
+// A reference maximum (base 2) beyond this is `far`.  The product logit * scale, less the reference, is one fused operation on the tensor
+// cores' kernels; the reference is a product rounded to fp32, so that the difference of the largest logit from itself is not zero but up
+// to half a unit of the reference's last place: 2^-8 here, a factor of 2^128 and more from 2^31 on.  Far logits are multiplied first.
+constexpr float kFar = 65536.f;
+__device__ __forceinline__ bool is_far(float ref) { return fabsf(ref) > kFar && fabsf(ref) != INFINITY; }
+
 __device__ __forceinline__ bool sees(const TreeParams& P, int b, int t, int u) {
   return P.mask != nullptr ? P.mask[b * P.m_sb + t * P.m_st + u] != 0 : u <= t;
 }
@@ -821,7 +827,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmKc, const __grid_constant__
           pair_sync();
           m = fmaxf(m, xchg[s][buf][half ^ 1][lane_row]);
         }
-        const float m2 = m * scale2;              // -inf: nothing seen
+        const float m2 = __fmul_rn(m, scale2);    // -inf: nothing seen
         bool need = false;
         float alpha = 1.f;
         if (m_ref == -INFINITY) {
@@ -847,11 +853,19 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmKc, const __grid_constant__
           tmem_st_wait();
         }
         const float ref = m_ref == -INFINITY ? 0.f : m_ref;     // -inf - -inf must not be formed
+        float by = scale2;
+        if (is_far(ref)) {
+#pragma unroll
+          for (int k = 0; k < NCH; ++k)
+#pragma unroll
+            for (int i = 0; i < CH; ++i) x[k][i] = __fmul_rn(x[k][i], scale2);
+          by = 1.f;
+        }
         if (STREAMS == 2 && turns && (s == 1 || u > 0)) my_turn();
 #pragma unroll
         for (int k = 0; k < NCH; ++k) {
           uint32_t r[CH / 2];
-          l += exp_pack_row(x[k], scale2, ref, r);       // a masked logit, -inf, gives 0
+          l += exp_pack_row(x[k], by, ref, r);       // a masked logit, -inf, gives 0
           if (STREAMS == 2 && turns && k == NCH - 1) your_turn();
           tmem_st_words(tP + half * (CW / 2) + k * 16, r);
         }
@@ -985,8 +999,8 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmKc, const __grid_constant__
 // sixteen columns each) and exponentials for the rows there are; P^T goes through shared memory, K-major as the products want it.
 //   * The reference maxima are one per column, the same for all threads, in shared memory.  While no logit exceeds its column's by
 //     more than 2^8 (one vote of all softmax warps a block) nothing is reduced over the keys; else, for the first block of a unit, for
-//     those behind it while a column has seen nothing but -inf, and for those of the drafted rows, the maxima are taken, O^T and the
-//     sums rescaled.
+//     those behind it while a column has seen nothing but -inf or has a far reference, and for those of the drafted rows, the maxima
+//     are taken, O^T and the sums rescaled.
 //   * Sums stay with the threads, a key each, until a unit ends.
 //   * The transposed accumulator leaves whole rows of the output side by side.
 // Against the tile with rows as rows and copies of them over the keys, calls back to back: one token over 4096 rows 12.3 -> 11.6 us, 32
@@ -1138,7 +1152,8 @@ tree_few_kernel(const __grid_constant__ CUtensorMap tmKc, const __grid_constant_
       float l[NT];
 #pragma unroll
       for (int c = 0; c < NT; ++c) l[c] = 0.f;
-      bool open = true;         // a column has no reference yet (all its logits were -inf): the same for all softmax warps
+      // a column has no reference yet (all its logits were -inf), or a far one: the same for all softmax warps
+      bool careful = true;
       for (int j = walk.j0; j < walk.j1; ++j, ++u) {
         const uint32_t buf = u & 1, phase = (u >> 1) & 1;
         const bool draft = j >= walk.cached;
@@ -1167,7 +1182,7 @@ tree_few_kernel(const __grid_constant__ CUtensorMap tmKc, const __grid_constant_
             unpack2(fma2(pack2(x[c + 2], x[c + 3]), scale, pack2(o.z, o.w)), y[c + 2], y[c + 3]);
           }
         };
-        bool renew = open || draft;
+        bool renew = careful || draft;
         if (!renew) {
           shift();
           renew = soft_any(max_row<NT>(y) > 8.f);
@@ -1180,14 +1195,15 @@ tree_few_kernel(const __grid_constant__ CUtensorMap tmKc, const __grid_constant_
           if (lane < NT) found[quarter][col0 + lane] = mine;
           soft_sync();
           if (tid < here) {
-            const float m2 = fmaxf(fmaxf(found[0][tid], found[1][tid]), fmaxf(found[2][tid], found[3][tid])) * scale2, old = ref[tid];
+            const float m = fmaxf(fmaxf(found[0][tid], found[1][tid]), fmaxf(found[2][tid], found[3][tid]));
+            const float m2 = __fmul_rn(m, scale2), old = ref[tid];
             const bool grown = old == -INFINITY ? m2 > old || m2 != m2 : m2 > old + 8.f;
             factor[tid] = grown && old != -INFINITY ? ex2(old - m2) : 1.f;
             if (grown) { ref[tid] = m2; off[tid] = -m2; }
           } else if (tid < N) {
             factor[tid] = 1.f;
           }
-          open = soft_any(tid < here && ref[tid] == -INFINITY);
+          careful = soft_any(tid < here && (ref[tid] == -INFINITY || is_far(ref[tid])));
 #pragma unroll
           for (int c = 0; c < NT; ++c) l[c] *= factor[col0 + c];
           if (j > walk.j0) {
@@ -1204,7 +1220,10 @@ tree_few_kernel(const __grid_constant__ CUtensorMap tmKc, const __grid_constant_
             }
             tmem_st_wait();
           }
-          shift();
+          if (!careful) shift();
+          else
+#pragma unroll
+            for (int c = 0; c < NT; ++c) y[c] = __fadd_rn(__fmul_rn(x[c], scale2), off[col0 + c]);
         }
 #pragma unroll
         for (int c = 0; c < NT; ++c) y[c] = ex2(y[c]);
