@@ -20,6 +20,7 @@ static std::vector<OptTensor> tree_attend(Tensor q, Tensor k_cache, Tensor v_cac
     require(t->device() == q.device() && t->scalar_type() == q.scalar_type(), "tensors must share device and type");
     for (int64_t s : t->sizes()) require(s <= 0x7fffffff, "a size is above 2^31");
     require(!at::GradMode::is_enabled() || !t->requires_grad(), "no gradient passes: call it under no_grad, or with detached tensors");
+    require(!t->_fw_grad(0).defined(), "no forward-mode derivative passes: call it with the tensors without their tangents");
   }
   const int64_t b = q.size(0), t = q.size(2), d = q.size(3), kv = k.size(1);
   require(k.size(0) == b && k.size(2) == t && k.size(3) == d && v.sizes() == k.sizes(),
