@@ -1,11 +1,11 @@
 // Rotation of queries and keys by their positions, with or without their norm: the call, and the autograd node around it.
 
-#include <ATen/MemoryOverlap.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/saved_variable.h>
 
 #include <algorithm>
+#include <initializer_list>
 
 #include "nsa_host.h"
 
@@ -60,16 +60,83 @@ nsa_heads_args head_args(const Rotation& r, const Tensor& like) {
   return a;
 }
 
-// A thread reads its part of a row before it writes it, so an output may be the tensor that it belongs to, and none of the others
-void check_output(const Tensor& out, const Tensor& own, const Tensor& other, const Tensor& other_out) {
-  using at::MemOverlapStatus;
-  auto shared = [&](const Tensor& t) {
-    const MemOverlapStatus s = at::get_overlap_status(out, t);
-    return s == MemOverlapStatus::Full || s == MemOverlapStatus::Partial;
-  };
-  require(at::has_internal_overlap(out) != at::MemOverlap::Yes, "an output must not be broadcast");
-  require(at::get_overlap_status(out, own) != MemOverlapStatus::Partial, "an output may be the tensor itself, but must not overlap it otherwise");
-  require((!other.defined() || !shared(other)) && (!other_out.defined() || !shared(other_out)), "an output of one of the tensors must not overlap the other's");
+// Do strided tensors meet in memory?  Addresses are base + sum index_k step_k, so they do if their bases' difference is a sum of
+// e_k step_k with every e_k between the bounds that the sizes set; axes are tried from the widest step down, each over the few numbers
+// that leave what the narrower ones can reach.  (ATen's own test answers for dense tensors alone, and neither some heads of a
+// projection nor some rows of a cache are dense.)
+struct Axis { int64_t step, lo, hi; };      // bytes
+
+class Sums {
+ public:
+  void add(int64_t step, int64_t lo, int64_t hi) {
+    if (step != 0 && lo != hi) axes_.push_back({step, lo, hi});
+  }
+  // Is there such a sum?  Also true where that is not found out within so many tries
+  bool reach(int64_t target) {
+    std::sort(axes_.begin(), axes_.end(), [](const Axis& a, const Axis& b) { return a.step > b.step; });
+    least_.assign(axes_.size() + 1, 0);
+    most_.assign(axes_.size() + 1, 0);
+    for (size_t k = axes_.size(); k-- > 0;) {
+      least_[k] = least_[k + 1] + axes_[k].lo * axes_[k].step;
+      most_[k] = most_[k + 1] + axes_[k].hi * axes_[k].step;
+    }
+    tries_ = 1 << 16;
+    return from(0, target);
+  }
+
+ private:
+  static int64_t floor_of(int64_t x, int64_t y) { return x / y - (x % y < 0); }
+  bool from(size_t k, int64_t target) {
+    if (target < least_[k] || target > most_[k]) return false;
+    if (k == axes_.size() || --tries_ < 0) return true;
+    const Axis& a = axes_[k];
+    const int64_t lo = std::max(a.lo, -floor_of(most_[k + 1] - target, a.step)), hi = std::min(a.hi, floor_of(target - least_[k + 1], a.step));
+    for (int64_t e = lo; e <= hi; ++e)
+      if (from(k + 1, target - e * a.step)) return true;
+    return false;
+  }
+  std::vector<Axis> axes_;
+  std::vector<int64_t> least_, most_;
+  int tries_ = 0;
+};
+
+bool meet(const Tensor& a, const Tensor& b) {
+  if (!a.defined() || !b.defined() || a.numel() == 0 || b.numel() == 0) return false;
+  Sums sums;
+  for (int64_t k = 0; k < a.dim(); ++k) sums.add(a.stride(k) * a.element_size(), 0, a.size(k) - 1);
+  for (int64_t k = 0; k < b.dim(); ++k) sums.add(b.stride(k) * b.element_size(), -(b.size(k) - 1), 0);
+  sums.add(1, -(int64_t)(b.element_size() - 1), a.element_size() - 1);
+  return sums.reach(reinterpret_cast<intptr_t>(b.data_ptr()) - reinterpret_cast<intptr_t>(a.data_ptr()));
+}
+
+// Do two elements of a tensor share memory?  Then their indices' first difference, along some axis, is positive for one of them
+bool meets_itself(const Tensor& t) {
+  if (t.numel() == 0) return false;
+  for (int64_t k = 0; k < t.dim(); ++k) {
+    if (t.size(k) <= 1) continue;
+    if (t.stride(k) == 0) return true;
+    Sums sums;
+    sums.add(t.stride(k) * t.element_size(), 0, t.size(k) - 2);
+    for (int64_t i = k + 1; i < t.dim(); ++i) sums.add(t.stride(i) * t.element_size(), -(t.size(i) - 1), t.size(i) - 1);
+    sums.add(1, -(int64_t)(t.element_size() - 1), t.element_size() - 1);
+    if (sums.reach(-t.stride(k) * (int64_t)t.element_size())) return true;
+  }
+  return false;
+}
+
+bool same_place(const Tensor& a, const Tensor& b) {
+  if (a.data_ptr() != b.data_ptr() || a.sizes() != b.sizes()) return false;
+  for (int64_t k = 0; k < a.dim(); ++k)
+    if (a.size(k) > 1 && a.stride(k) != b.stride(k)) return false;
+  return true;
+}
+
+// A thread reads its part of a row before it writes it, so an output may be the tensor that it belongs to, and nothing else that is read
+void check_output(const Tensor& out, const Tensor& own, const Tensor& other, const Tensor& other_out, std::initializer_list<Tensor> read) {
+  require(!meets_itself(out), "an output must not be broadcast, nor overlap itself");
+  require(same_place(out, own) || !meet(out, own), "an output may be the tensor itself, but must not overlap it otherwise");
+  require(!meet(out, other) && !meet(out, other_out), "an output of one of the tensors must not overlap the other's");
+  for (const Tensor& t : read) require(!meet(out, t), "an output must not overlap the weights, the positions or the frequencies");
   require(!at::GradMode::is_enabled() || !out.requires_grad(), "an output that wants gradients itself cannot be given");
 }
 
@@ -214,7 +281,7 @@ static std::vector<OptTensor> rotate_heads(Tensor q, OptTensor k_, OptTensor wq,
               "an output must have the tensor's device, type and shape, and a contiguous last axis");
   }
   for (int i = 0; i < 2; ++i)
-    if (given[i].defined()) check_output(given[i], x[i], x[1 - i], given[1 - i]);
+    if (given[i].defined()) check_output(given[i], x[i], x[1 - i], given[1 - i], {w[0], w[1], positions.value_or(Tensor()), steps});
   wanted = wanted && at::GradMode::is_enabled();
   require(!wanted || (!given[0].defined() && !given[1].defined()), "outputs cannot be given where gradients are wanted");
   if (positions.has_value() && positions->defined()) {
@@ -279,6 +346,9 @@ static std::vector<OptTensor> rotate_heads(Tensor q, OptTensor k_, OptTensor wq,
 
 void bind_heads(pybind11::module_& m) {
   m.def("rotate_heads", &rotate_heads, pybind11::call_guard<pybind11::gil_scoped_release>());
+  // what outputs are checked by, on any tensors
+  m.def("tensors_meet", &meet);
+  m.def("tensor_meets_itself", &meets_itself);
 }
 
 }  // namespace nsa_host
