@@ -233,7 +233,8 @@ Gradients RotatedHeadsBackward::heads_backward(const Rotation& r, const Tensor* 
     if (r.norm) {
       a.part[i].x = t4(x[i]);
       set_weight(a, i, w[i], x[i]);
-      g.dw[i] = at::empty(w[i].sizes(), w[i].options());
+      // (a tensor without heads is not there for the kernels)
+      g.dw[i] = x[i].size(1) > 0 ? at::empty(w[i].sizes(), w[i].options()) : at::zeros(w[i].sizes(), w[i].options());
       a.part[i].dweight = g.dw[i].data_ptr();
     }
   }
