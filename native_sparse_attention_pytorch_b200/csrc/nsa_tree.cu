@@ -27,11 +27,13 @@ __device__ __forceinline__ int length_of(const TreeParams& P, int b) {
   return max(0, min(n, P.capacity));
 }
 
-// Key blocks of one KV head of a sequence
+// Key blocks of one KV head of a sequence.  (Unsigned: a length may lie less than a block below 2^31.)
 template <int KB>
-__device__ __forceinline__ int cache_blocks(const TreeParams& P, int b) { return (length_of(P, b) + KB - 1) / KB; }
+__device__ __forceinline__ int blocks_of(int rows) { return (int)(((unsigned)rows + KB - 1) / KB); }
 template <int KB>
-__device__ __forceinline__ int draft_blocks(const TreeParams& P) { return (P.tokens + KB - 1) / KB; }
+__device__ __forceinline__ int cache_blocks(const TreeParams& P, int b) { return blocks_of<KB>(length_of(P, b)); }
+template <int KB>
+__device__ __forceinline__ int draft_blocks(const TreeParams& P) { return blocks_of<KB>(P.tokens); }
 
 // Blocks of the units of the sequences before `upto`, and of all, by a whole warp
 template <int KB>
@@ -541,7 +543,7 @@ struct Walk {
   __device__ void ask(const TreeParams& P, int lane) { length = lane < P.batch ? length_of(P, lane) : 0; }
   __device__ void begin(const TreeParams& P, int lane, int group) {
     if (P.batch <= 32) {                  // one look at the lengths
-      const int64_t n = lane < P.batch ? ((int64_t)(length + KB - 1) / KB + draft_blocks<KB>(P)) * P.kv_heads : 0;
+      const int64_t n = lane < P.batch ? ((int64_t)blocks_of<KB>(length) + draft_blocks<KB>(P)) * P.kv_heads : 0;
       int64_t upto = n;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -570,7 +572,7 @@ struct Walk {
   __device__ bool unit(const TreeParams& P) {
     if (at >= end) return false;
     length = length_of(P, b);
-    cached = (length + KB - 1) / KB;
+    cached = blocks_of<KB>(length);
     per_unit = cached + draft_blocks<KB>(P);
     h = (int)quotient(at - base, per_unit);
     unit0 = base + (int64_t)h * per_unit;
