@@ -685,6 +685,8 @@ static int fill_heads(HeadsParams& P, const nsa_heads_args& a, bool backward) {
   if (a.rotary_dim < 2 || a.rotary_dim % 2 || a.rotary_dim > a.dim_head)
     return fail(NSA_ERR_SHAPE, "heads: rotary_dim must be even, at least 2 and at most dim_head");
   if ((int64_t)a.batch * a.seq > 0x7fffffffLL) return fail(NSA_ERR_SHAPE, "heads: batch * seq must stay below 2^31");
+  if ((int64_t)a.part[0].heads + a.part[1].heads > 0x7fffffffLL - 64)      // slots of 32 heads are rounded up
+    return fail(NSA_ERR_SHAPE, "heads: queries and keys must have fewer than 2^31 - 64 heads together");
   memset(&P, 0, sizeof(P));
   P.batch = a.batch; P.seq = a.seq; P.d = a.dim_head; P.rotary_dim = a.rotary_dim; P.half = a.half != 0;
   P.norm = a.norm != 0; P.weight_f32 = a.weight_f32 != 0; P.weight_per_head = a.weight_per_head != 0;

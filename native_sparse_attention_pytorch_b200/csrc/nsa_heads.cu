@@ -275,7 +275,7 @@ __global__ void __launch_bounds__(heads::kThreads, heads::kBlocksPerSM) heads_ke
 
   const unsigned tokens = (unsigned)P.batch * (unsigned)P.seq;
   const float inv_d = 1.f / (float)P.d;
-  const unsigned step = blocks * groups;
+  const unsigned step = (unsigned)blocks * groups, begin = (unsigned)at_block * groups;
   auto position = [&](unsigned token) {
     const unsigned b = token / (unsigned)P.seq, n = token - b * (unsigned)P.seq;
     if (P.positions == nullptr) return P.offset + n;
@@ -289,7 +289,7 @@ __global__ void __launch_bounds__(heads::kThreads, heads::kBlocksPerSM) heads_ke
 
   // RING: rows are on their way kStages - 1 heads ahead, past the end of a token into the next one
   const uint32_t place = ptx::smem_u32(places + threadIdx.x);
-  unsigned far_token = at_block * groups + group;
+  unsigned far_token = begin + group;
   int far_head = h0, far_stage = 0, stage = 0;
   const T *far_x = nullptr, *far_g = nullptr;
   auto far_locate = [&]() {
@@ -323,10 +323,10 @@ __global__ void __launch_bounds__(heads::kThreads, heads::kBlocksPerSM) heads_ke
 #pragma unroll 1
     for (int i = 0; i < kStages - 1; ++i) far_fetch();
   }
-  int64_t next_pos = position(min(at_block * groups + group, tokens - 1));
+  int64_t next_pos = position(min(begin + group, tokens - 1));
 
   // every lane of a warp takes part in the sums over a row: groups without a token go along with nothing to load
-  for (unsigned first = at_block * groups; first < tokens; first += step) {
+  for (unsigned first = begin; first < tokens; first += step) {
     const unsigned token = first + group;
     const bool live = token < tokens;
     const T* xp = XIN && !RING ? row_at(R.x, R.x_sb, R.x_sh, R.x_sn, live ? token : 0) : nullptr;
