@@ -676,6 +676,8 @@ int nsa_rmsnorm_bwd(const nsa_rmsnorm_bwd_args* a, void* stream) {
   return launch_rmsnorm(P, a->fwd.dtype, true, (cudaStream_t)stream);
 }
 
+static bool off_boundary(const void* p, uintptr_t size) { return (reinterpret_cast<uintptr_t>(p) & (size - 1)) != 0; }
+
 static int fill_heads(HeadsParams& P, const nsa_heads_args& a, bool backward) {
   if (a.dtype != NSA_F32 && a.dtype != NSA_BF16) return fail(NSA_ERR_DTYPE, "dtype must be NSA_F32 or NSA_BF16");
   if (a.batch < 0 || a.seq < 0 || a.part[0].heads < 0 || a.part[1].heads < 0)
@@ -694,6 +696,8 @@ static int fill_heads(HeadsParams& P, const nsa_heads_args& a, bool backward) {
   P.steps = a.steps; P.magnitude = a.magnitude; P.eps = a.eps;
   const bool rows = (int64_t)a.batch * a.seq > 0;
   if (rows && a.steps == nullptr) return fail(NSA_ERR_NULL, "heads: steps is NULL");
+  if (off_boundary(a.steps, 8) || off_boundary(a.positions, a.pos_i64 ? 8 : 4))
+    return fail(NSA_ERR_ALIGN, "heads: steps or positions do not start on a boundary of their type");
   const uintptr_t unit = a.dtype == NSA_F32 ? 3 : 1;
   for (int i = 0; i < 2; ++i) {
     const nsa_head_rows& r = a.part[i];
@@ -703,6 +707,9 @@ static int fill_heads(HeadsParams& P, const nsa_heads_args& a, bool backward) {
     R.weight = r.weight; R.dweight = r.dweight;
     if (a.norm && (rows && r.weight == nullptr)) return fail(NSA_ERR_NULL, "heads: weight is NULL");
     if (a.norm && backward && r.dweight == nullptr) return fail(NSA_ERR_NULL, "heads: dweight is NULL");
+    const uintptr_t weight_size = a.weight_f32 ? 4 : unit + 1;
+    if (a.norm && (off_boundary(r.weight, weight_size) || (backward && off_boundary(r.dweight, weight_size))))
+      return fail(NSA_ERR_ALIGN, "heads: a weight does not start on a boundary of its type");
     if (!rows) continue;
     const bool reads_x = !backward || a.norm;
     if (r.out.ptr == nullptr || (reads_x && r.x.ptr == nullptr) || (backward && r.dy.ptr == nullptr))
@@ -759,6 +766,8 @@ static int fill_tree(TreeParams& P, const nsa_tree_args& a) {
   P.G = a.q_heads / a.kv_heads; P.scale = a.scale; P.length = a.length; P.lengths = a.lengths;
   P.mask = a.mask; P.m_sb = a.mask_stride_b; P.m_st = a.mask_stride_t; P.lse = a.lse;
   if ((int64_t)a.batch * a.tokens == 0) return NSA_OK;
+  if (off_boundary(a.lengths, 4) || off_boundary(a.lse, 4) || off_boundary(a.status, 4))
+    return fail(NSA_ERR_ALIGN, "tree: lengths, lse or status do not start on a boundary of their type");
   const nsa_tensor* all[] = {&a.q, &a.k, &a.v, &a.out, &a.k_cache, &a.v_cache};
   const uintptr_t unit = a.dtype == NSA_F32 ? 3 : 1;
   for (int i = 0; i < (a.capacity > 0 ? 6 : 4); ++i) {
