@@ -555,8 +555,8 @@ int nsa_decode_step(const nsa_decode_args* args, void* stream);
  * at the angle positions[b, i] + offset times the pair's frequency; pairs are
  * (2m, 2m+1), or (m, m + rotary_dim/2) with `half`; features from rotary_dim
  * on pass unchanged.  A frequency is given as the 64-bit fraction of a turn
- * per position (steps[m] = 2^64 * frequency / 2 pi, rounded), so that angles
- * stay exact at any int64 position.  Any element strides; rows need no
+ * per position (steps[m] = 2^64 * frequency / 2 pi, rounded); the multiples of
+ * that fraction are exact at any int64 position.  Any element strides; rows need no
  * alignment beyond their type's (16-byte aligned ones are moved fastest).
  * The backward writes dx to `out` and, with norm, the weights' gradients in
  * the weights' type, in a fixed order of summation.  `out` may be x itself

@@ -4,8 +4,9 @@
 // R turns the first `rotary_dim` features pair by pair and multiplies them with a magnitude; the others pass as they are.
 //
 // Angles.  A frequency is held as a 64-bit fraction of a turn per position, so position times frequency is an integer
-// product whose overflow drops whole turns: the phase is exact to pos * 2^-65 turns, where a product in fp32 is off by 0.03
-// radians at position 10^6.  Sines and cosines of it are good to 10^-7 at any position.
+// product whose overflow drops whole turns: nothing is lost but what the fraction itself is off by (2^-52 of a frequency that was a
+// double: 2^-52 radians a position at most, 10^-7 at 4 * 10^8), where a product in fp32 is off by 0.03 radians at position 10^6.  Sines
+// and cosines of the phase are good to 2 * 10^-7 at any position.
 // Angles are formed in the kernel: one set per token serves all its heads, so there is no table to build, keep or read.
 //
 // Work.  A row (one head of one token) belongs to 2^k neighbouring lanes, a lane to `units` of two vectors of W elements, whose

@@ -113,8 +113,9 @@ class RotaryFrequencies:
     frequencies   instead of theta and scaling: rotary_dim / 2 radians per position
     magnitude     factor on the rotated features, instead of the scaling's own
 
-    Frequencies are computed in 64 bits and kept as 64-bit fractions of a turn, so that angles are exact at any position
-    (`module.bfloat16()` of whatever holds this changes nothing)."""
+    Frequencies are doubles, kept as 64-bit fractions of a turn (`module.bfloat16()` of whatever holds this changes nothing).  An angle
+    is off by the rounding of that fraction alone, |position| * (|frequency| * 2^-52 + 2^-62) radians at most: 10^-7 at position
+    4 * 10^8 for a frequency of 1, less for lower ones."""
 
     def __init__(self, dim_head, rotary_dim=None, theta=10000.0, layout='interleaved', scaling=None, factor=1.0,
                  original_length=None, beta_fast=32.0, beta_slow=1.0, frequencies=None, magnitude=None):
