@@ -12,10 +12,11 @@
 // Work.  A row (one head of one token) belongs to 2^k neighbouring lanes, a lane to `units` of two vectors of W elements, whose
 // elements are W pairs (u, v): with the half layout u from one vector and v from the other, else even and odd elements of both.
 // A group of lanes goes through up to `per_slot` heads of a token (a slot: heads of the queries or of the keys), kBatch of them in
-// flight, two values an instruction.  What bounds it is the
-// traffic: x (and dy) in, y (or dx) out.  bf16: rotation of 65536 x 72 heads of 128 365 us, 6.6 TB/s (the copy's rate); with the norm 16383 x 72 of
-// 128 100 us, 6.1 TB/s; its backward for 32768 x 36 of 64 81 us, 5.6 TB/s, half of the issue slots busy with 16 warps an SM.
-// With the norm, rows come through thread-private places in shared memory, some heads ahead: registers go to the factors.
+// flight, two values an instruction.  With the norm, rows come through thread-private places in shared memory, some heads ahead:
+// registers go to the factors.
+// What bounds it is the traffic: x (and dy) in, y (or dx) out.  bf16: rotation of 65536 x 72 heads of 128 365 us, 6.6 TB/s (the copy's
+// rate); with the norm 16383 x 72 of 128 100 us, 6.1 TB/s; its backward for 32768 x 36 of 64 81 us, 5.6 TB/s, half of the issue slots
+// busy with 16 warps an SM.
 
 #include "nsa_common.cuh"
 #include "nsa_kernels.h"

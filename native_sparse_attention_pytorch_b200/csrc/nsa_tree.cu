@@ -11,8 +11,10 @@
 // per CTA: slot 0 where the piece begins inside the unit, slot 1 where it begins with it.  tree_merge_kernel joins a unit's
 // partials, whose groups follow from the same arithmetic, in the order of the keys.
 //
-// Rows behind a length are never read.  A drafted value that is not finite would reach tokens which do not see it (0 times
-// infinity is NaN): such values are left out of the products, and added behind them for the tokens that see them.
+// Rows behind a length leave no trace.  The CUDA cores do not read them; the tensor cores' kernels fetch a sequence's last block whole,
+// mask the logits of the rows behind and clear their values before the products.  A drafted value that is not finite would reach
+// tokens which do not see it (0 times infinity is NaN): such values are left out of the products, and added behind them for the
+// tokens that see them.
 
 #include "nsa_common.cuh"
 #include "nsa_kernels.h"
@@ -156,8 +158,9 @@ __device__ __forceinline__ const T* row_of(const RowView& r, int b, int h, int64
 // ---- any type and alignment, on the CUDA cores -------------------------------------------
 
 // fp32, and bf16 rows that TMA cannot fetch.  256 threads share a tile of 8, 32 or 64 rows: scores of a block into shared memory, softmax
-// by 32, 8 or 4 lanes a row, values times weights in registers.  Bound by shared memory and issue: with 64 rows a thread has 4 rows x 2
-// keys, then 4 x 8 columns, eight and nine 16-byte reads for 32 and 128 fused multiplications of a step.  fp32 rows arrive a block ahead.
+// by 32, 8 or 4 lanes a row, values times weights in registers.  Bound by shared memory and issue: with 64 rows of 128 a thread has 4 rows
+// x 2 keys and four features, then 4 x 8 columns and four keys: six and twelve 16-byte reads for 32 and 128 fused multiplications of a
+// step.  fp32 rows arrive a block ahead.
 // 4 x 64 tokens over 4096 rows, 64 / 8 heads of 128: 977 us, 30 TFLOP/s (tiles of 32 rows, loads in turn, columns read one by one: 1712);
 // 16 x one token over 8192 rows, 32 / 4 heads of 128: 126 us, 3.2 TB/s (two rows x one key a thread: 167).
 
@@ -502,8 +505,8 @@ __global__ void __launch_bounds__(tree_simt::kThreads, tree_simt::Shape<DP, RT>:
 //   MMA warp(s)     S = Q K^T, then O += P V with P from tensor memory; one per stream
 //   softmax warps   S from tensor memory, maximum, exponentials, P back as bf16.  A warp reaches 32 lanes of tensor memory, 32 rows.
 //                   One stream: two threads per row, half of a block's keys each, which exchange maxima.  Two streams: one thread (64
-//                   tokens over 65536 rows, a block of 64 keys and two tiles: 1790 cycles, with two threads 2000).  P is rounded (2^-9 on average a weight, as any bf16 tensor of
-//                   weights would be); the sum adds the exponentials as they are.
+//                   tokens over 65536 rows, a block of 64 keys and two tiles: 1790 cycles, with two threads 2000).  P is rounded, up to
+//                   2^-8 of a weight, as any bf16 tensor of weights would be; the sum adds the exponentials as they are.
 // The accumulator O stays in tensor memory.  It is rescaled lazily: a row keeps its reference maximum until a block exceeds it by
 // more than 2^8.
 // What bounds it: the exponentials (16 a cycle and SM) and what else a warp does for a value beside them; then power.  64 tokens over 65536

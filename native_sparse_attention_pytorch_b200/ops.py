@@ -719,9 +719,9 @@ def tree_attend(q, k_cache, v_cache, lengths, k, v, mask=None, *, scale=None, re
     all).  mask: bool [t, t] or [b, t, t], mask[.., i, j]: token i sees drafted token j (a tree: its ancestors and itself);
     None: j <= i.  Every token sees all cached rows.  A token that sees nothing gets zeros and lse -inf; what lies behind a
     length, or in a drafted row that a token does not see, leaves no trace in it, NaN included.  scale defaults to
-    d^-0.5.  No gradient passes: tensors that want one are refused outside no_grad, those with a tangent always.  Returns out [b, q_heads, t, d], with
-    `return_lse` also its log sum of exponentials (fp32 [b, q_heads, t]), by which it can be merged with attention over other
-    keys.  See nsa_tree_attend in include/nsa_b200.h."""
+    d^-0.5.  No gradient passes: tensors that want one are refused outside no_grad, those with a tangent always.  Returns out
+    [b, q_heads, t, d], with `return_lse` also its log sum of exponentials (fp32 [b, q_heads, t]), by which it can be merged with
+    attention over other keys.  See nsa_tree_attend in include/nsa_b200.h."""
     length = 0
     if lengths is None:
         length = k_cache.shape[2]
