@@ -843,34 +843,38 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmKc, const __grid_constant__
           l *= alpha;
           need = true;
         }
-        if (j > walk.j0 && __any_sync(kFullMask, need)) {
-          mbar_wait_warp(smem_u32(&bars.pv_done[s][(u - 1) % LOOK]), ((u - 1) / LOOK) & 1, &abort_flag);
-          tc_fence_after_sync();
+        float ref = m_ref == -INFINITY ? 0.f : m_ref;     // -inf - -inf must not be formed
+        const bool far = is_far(ref);
+        // both are rare and share a branch (far ones in one of their own: 64 tokens over 65536 rows 1.6 % slower, so 0.5 %)
+        if (__any_sync(kFullMask, need || far)) {
+          if (__any_sync(kFullMask, need)) {        // not in a unit's first block: there the reference was -inf
+            mbar_wait_warp(smem_u32(&bars.pv_done[s][(u - 1) % LOOK]), ((u - 1) / LOOK) & 1, &abort_flag);
+            tc_fence_after_sync();
 #pragma unroll 1
-          for (int c = half * (D / HALVES); c < (half + 1) * (D / HALVES); c += 16) {
-            float o[16];
-            tmem_ld16(tm_lane + tO + c, o);
-            tmem_ld_wait();
+            for (int c = half * (D / HALVES); c < (half + 1) * (D / HALVES); c += 16) {
+              float o[16];
+              tmem_ld16(tm_lane + tO + c, o);
+              tmem_ld_wait();
 #pragma unroll
-            for (int i = 0; i < 16; ++i) o[i] *= alpha;
-            tmem_st16(tm_lane + tO + c, o);
+              for (int i = 0; i < 16; ++i) o[i] *= alpha;
+              tmem_st16(tm_lane + tO + c, o);
+            }
+            tmem_st_wait();
           }
-          tmem_st_wait();
-        }
-        const float ref = m_ref == -INFINITY ? 0.f : m_ref;     // -inf - -inf must not be formed
-        float by = scale2;
-        if (is_far(ref)) {
+          if (far) {          // multiplied, less the reference, and back to what the exponentials multiply
+            const float back = 1.f / scale2;
 #pragma unroll
-          for (int k = 0; k < NCH; ++k)
+            for (int k = 0; k < NCH; ++k)
 #pragma unroll
-            for (int i = 0; i < CH; ++i) x[k][i] = __fmul_rn(x[k][i], scale2);
-          by = 1.f;
+              for (int i = 0; i < CH; ++i) x[k][i] = __fmul_rn(__fsub_rn(__fmul_rn(x[k][i], scale2), ref), back);
+            ref = 0.f;
+          }
         }
         if (STREAMS == 2 && turns && (s == 1 || u > 0)) my_turn();
 #pragma unroll
         for (int k = 0; k < NCH; ++k) {
           uint32_t r[CH / 2];
-          l += exp_pack_row(x[k], by, ref, r);       // a masked logit, -inf, gives 0
+          l += exp_pack_row(x[k], scale2, ref, r);       // a masked logit, -inf, gives 0
           if (STREAMS == 2 && turns && k == NCH - 1) your_turn();
           tmem_st_words(tP + half * (CW / 2) + k * 16, r);
         }
