@@ -161,8 +161,9 @@ __device__ __forceinline__ const T* row_of(const RowView& r, int b, int h, int64
 // by 32, 8 or 4 lanes a row, values times weights in registers.  Bound by shared memory and issue: with 64 rows of 128 a thread has 4 rows
 // x 2 keys and four features, then 4 x 8 columns and four keys: six and twelve 16-byte reads for 32 and 128 fused multiplications of a
 // step.  fp32 rows arrive a block ahead.
-// 4 x 64 tokens over 4096 rows, 64 / 8 heads of 128: 977 us, 30 TFLOP/s (tiles of 32 rows, loads in turn, columns read one by one: 1712);
-// 16 x one token over 8192 rows, 32 / 4 heads of 128: 126 us, 3.2 TB/s (two rows x one key a thread: 167).
+// 4 x 64 tokens over 4096 rows, 64 / 8 heads of 128: 1111 us, 31 TFLOP/s (over half to all of them: 967; tiles of 32 rows, loads in turn,
+// columns read one by one: 1712); 16 x one token over 8192 rows, 32 / 4 heads of 128: 162 us, 3.3 TB/s (over half to all of them: 127; two
+// rows x one key a thread: 167).
 
 namespace tree_simt {
 constexpr int kThreads = 256;
@@ -510,7 +511,7 @@ __global__ void __launch_bounds__(tree_simt::kThreads, tree_simt::Shape<DP, RT>:
 // The accumulator O stays in tensor memory.  It is rescaled lazily: a row keeps its reference maximum until a block exceeds it by
 // more than 2^8.
 // What bounds it: the exponentials (16 a cycle and SM) and what else a warp does for a value beside them; then power.  64 tokens over 65536
-// rows, 64 / 8 heads of 128: 388 us, 1190 TFLOP/s, in bursts of 30 passes, 460 us back to back (1.5 GHz at 990 W).
+// rows, 64 / 8 heads of 128: 393 us, 1170 TFLOP/s, in bursts of 30 passes, 461 us back to back (1.5 GHz at 990 W).
 // STREAMS.  Above 128 rows two tiles share the K and V blocks; the softmax of one runs under the products of the other.  Blocks of 64
 // keys, so that tensor memory holds two S buffers of either beside both O: with blocks of 128 and one buffer, S of the next block
 // waited for the products of this one, which waited for its softmax (3800 cycles a block and pair of tiles, 2050 of them products).
