@@ -37,3 +37,5 @@ def test_on_the_tensor_cores():
     for t in (1, 20, 60, 100, 200):
         check(torch.zeros(1, 1, t, 64, device=DEV, dtype=torch.bfloat16), cache, t, MOST, 'sm100')
     check(torch.zeros(1, 1, 1, 64, device=DEV, dtype=torch.bfloat16), cache, 1, torch.tensor([MOST - 60], device=DEV), 'sm100')
+    del flat, cache
+    torch.cuda.empty_cache()
