@@ -27,6 +27,9 @@ void require(bool ok, const std::string& what) {
 // The last axis next to itself; the kernels take any other strides
 Tensor dense_rows(const Tensor& t) { return t.size(3) == 1 || t.stride(3) == 1 ? t : t.contiguous(); }
 
+// A view that PyTorch negates when it is read (the imaginary part of a conjugate) as values that lie in memory; its gradient passes
+Tensor plain(const Tensor& t) { return t.defined() && t.is_neg() ? t.resolve_neg() : t; }
+
 void check_rows(const Tensor& t, const char* name, const Tensor& like, const Rotation& r) {
   require_cuda(t);
   require(t.dim() == 4, std::string(name) + " must be [batch, heads, seq, dim_head]");
@@ -224,7 +227,7 @@ Gradients RotatedHeadsBackward::heads_backward(const Rotation& r, const Tensor* 
   for (int i = 0; i < 2; ++i) {
     if (sizes[i].empty() || !dy[i].defined()) continue;
     g.dx[i] = empty_in_order(sizes[i], strides[i], options);
-    rows[i] = dense_rows(dy[i]);
+    rows[i] = dense_rows(plain(dy[i]));
     if (!begun) a = head_args(r, g.dx[i]);
     begun = true;
     a.part[i].heads = g.dx[i].size(1);
@@ -256,7 +259,8 @@ static std::vector<OptTensor> rotate_heads(Tensor q, OptTensor k_, OptTensor wq,
                                            OptTensor out_q, OptTensor out_k) {
   Rotation r;
   r.steps = steps; r.rotary_dim = rotary_dim; r.half = half; r.magnitude = magnitude; r.offset = offset; r.norm = norm; r.eps = eps;
-  Tensor x[2] = {q, k_.value_or(Tensor())}, w[2] = {wq.value_or(Tensor()), wk.value_or(Tensor())};
+  q = plain(q);
+  Tensor x[2] = {q, plain(k_.value_or(Tensor()))}, w[2] = {plain(wq.value_or(Tensor())), plain(wk.value_or(Tensor()))};
   Tensor given[2] = {out_q.value_or(Tensor()), out_k.value_or(Tensor())};
   bool wanted = false;
   require_cuda(q);
@@ -278,8 +282,8 @@ static std::vector<OptTensor> rotate_heads(Tensor q, OptTensor k_, OptTensor wq,
     }
     if (given[i].defined())
       require(given[i].device() == x[i].device() && given[i].scalar_type() == x[i].scalar_type() && given[i].sizes() == x[i].sizes() &&
-                  (x[i].size(3) == 1 || given[i].stride(3) == 1),
-              "an output must have the tensor's device, type and shape, and a contiguous last axis");
+                  (x[i].size(3) == 1 || given[i].stride(3) == 1) && !given[i].is_neg(),
+              "an output must have the tensor's device, type and shape, a contiguous last axis, and not be negated");
   }
   for (int i = 0; i < 2; ++i)
     if (given[i].defined()) check_output(given[i], x[i], x[1 - i], given[1 - i], {w[0], w[1], positions.value_or(Tensor()), steps});

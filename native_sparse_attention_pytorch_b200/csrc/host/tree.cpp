@@ -32,6 +32,9 @@ static std::vector<OptTensor> tree_attend(Tensor q, Tensor k_cache, Tensor v_cac
   const at::NoGradGuard no_grad;
   auto dense = [](const Tensor& x) { return x.size(3) == 1 || x.stride(3) == 1 ? x : x.contiguous(); };
   require(k_cache.stride(3) == 1 && v_cache.stride(3) == 1, "the caches' last axis must be contiguous");
+  require(!k_cache.is_neg() && !v_cache.is_neg(), "the caches must not be views that are negated when read");
+  for (Tensor* t : {&q, &k, &v})
+    if (t->is_neg()) *t = t->resolve_neg();
   q = dense(q);
   k = q.scalar_type() == at::kBFloat16 ? rowwise(k) : dense(k);
   v = q.scalar_type() == at::kBFloat16 ? rowwise(v) : dense(v);
